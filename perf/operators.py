@@ -390,7 +390,7 @@ def _held(s):
         elif c["kind"] == "scored":
             need = m.scored_workspace_bytes(s["cache"], c["q_heads"], c["batch"], c["tokens"], s["max_context"])
         else:
-            need = m.evict_workspace_bytes(s["cache"], c["batch"], s["max_context"], c["budget"])
+            need = 0  # eviction needs none
         s["ws"] = torch.empty(max(need, 1), dtype=torch.uint8, device=DEV)
     return m, s["cache"], s["ws"]
 
@@ -405,7 +405,7 @@ def _own(s):
     if c["kind"] == "evict":
         m.evict(cache, s["weights"], s["lengths"], budget=c["budget"], sinks=c["sinks"], recent=c["recent"],
                 max_context=s["max_context"], dst_table=s["dst"], kept=s["kept"], new_lengths=s["new_lengths"],
-                weights_out=s["weights_out"], workspace=ws)
+                weights_out=s["weights_out"])
         return _evicted(s)
     outs = {"gate": s["gate"], "gated_out": s["out"]} if c["gate"] else {"out": s["out"]}
     if c["kind"] == "window":
