@@ -366,6 +366,79 @@ miikv_status miikv_suffix_attn_ex(const miikv_view* view, const uint16_t* k_new,
                                   const float* gate, float* gated_out, void* workspace,
                                   uint64_t workspace_bytes, void* stream);
 
+/* ---- attention over part of a cache ---------------------------------------- */
+
+/* What a token sees: the token at position p of a sequence sees the keys j <= p with
+ * j > p - window (window == 0: all of them) or j < sinks, the sequence's first keys,
+ * which stay visible however far the window moves.  A token that sees no key (one of
+ * a context shorter than its tokens) gets zeros.  Pages whose keys no token of the
+ * call sees are not read: their table entries may be -1.  No counterpart in the
+ * reference, whose attention layers see the whole context. */
+
+/* Decode attention with a sliding window: the last `tokens` tokens of each sequence
+ * (1: a decode step; more: drafted tokens being verified), whose rows the cache holds.
+ *   q    device [batch][tokens][q_heads][head_dim], fp16 or fp32; tokens * q_heads /
+ *        kv_heads <= 16 (else MIIKV_EUNSUPPORTED)
+ *   context length of sequence b, its new tokens included: d_lengths[b], or
+ *        decode_state->position + 1 (batch must be 1); values above max_context count
+ *        as max_context
+ *   out / gated_out  device fp32, as q; gated_out = out * sigmoid(gate), gate and
+ *        gated_out go together.  At least one output is required.
+ * Outputs hold fp32's precision: key codes enter exactly, block scales are applied in
+ * fp32, an fp32 query and the probabilities as two fp16 parts.  All pointers 16-byte
+ * aligned (else MIIKV_EINVAL).  The workspace needs no initialisation; calls that may
+ * overlap need workspaces of their own.  miikv_window_workspace_bytes() is 0 for
+ * arguments that the call refuses. */
+uint64_t miikv_window_workspace_bytes(const miikv_view* view, uint32_t q_heads, uint32_t batch, uint32_t tokens,
+                                      uint32_t max_context, uint32_t window, uint32_t sinks);
+miikv_status miikv_decode_attn_window(const miikv_view* view, const void* q, uint32_t q_dtype, uint32_t q_heads,
+                                      float scale, uint32_t batch, uint32_t tokens, const uint32_t* d_lengths,
+                                      const miikv_decode_state* decode_state, uint32_t max_context, uint32_t window,
+                                      uint32_t sinks, float* out, const float* gate, float* gated_out, void* workspace,
+                                      uint64_t workspace_bytes, void* stream);
+
+/* Decode attention over the whole context that adds up what every key is worth:
+ * key_weights[b][h][j] += the sum, over the call's tokens of sequence b and the query
+ * heads of kv head h, of key j's probability.  key_weights is device fp32
+ * [batch][kv_heads][weight_stride], weight_stride >= max_context; entries at or past a
+ * sequence's length stay as they are, so a row starts as zeros and grows with the
+ * cache.  Sums are made in a fixed order: the same inputs give the same bits.  Other
+ * arguments as miikv_decode_attn_window. */
+uint64_t miikv_scored_workspace_bytes(const miikv_view* view, uint32_t q_heads, uint32_t batch, uint32_t tokens,
+                                      uint32_t max_context);
+miikv_status miikv_decode_attn_scored(const miikv_view* view, const void* q, uint32_t q_dtype, uint32_t q_heads,
+                                      float scale, uint32_t batch, uint32_t tokens, const uint32_t* d_lengths,
+                                      const miikv_decode_state* decode_state, uint32_t max_context, float* key_weights,
+                                      uint64_t weight_stride, float* out, const float* gate, float* gated_out,
+                                      void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Eviction: of every (sequence, kv head) whose context is longer than `budget`, keep the
+ * first `sinks` keys, the last `recent` ones and, of those between, the ones with the
+ * largest key_weights (of equal ones the first; a NaN counts as less than any number),
+ * `budget` in all (sinks + recent <= budget), and move their rows, in order, to
+ * positions 0, 1, ...  Codes and scales move as they are.  A kept key keeps the rotation
+ * of the position it was stored at, so from here on a row's place in the cache is not
+ * its position: rows appended later come already rotated (miikv_append_f16,
+ * miikv_append_batch_f16, the fp16 fused calls, miikv_append_f32 without a norm weight).
+ *   kept          device int32 [batch][kv_heads][budget]: the positions that stayed,
+ *                 ascending; -1 past the new length
+ *   d_new_lengths device [batch]: min(length, budget); may be d_lengths
+ *   dst_table     NULL: the rows move within the sequence's own pages, which no other
+ *                 sequence (of the call, a fork or a saved prefix) may share.  Otherwise
+ *                 device int32 [batch][dst_stride]: pages of the same planes that none
+ *                 of the batch's sequences uses; every sequence's kept rows are written
+ *                 there, the old pages stay as they are (paged caches only).
+ *   weights_out   nullable; the kept keys' weights, [batch][kv_heads][weights_out_stride].
+ *                 May be key_weights (with the same stride): what lay between the new
+ *                 and the old length is zeroed then.  Otherwise entries past the new
+ *                 length stay as they are.
+ * Rows of the cache past the new length stay as they were (in place: as the move left
+ * them).  No counterpart in the reference. */
+miikv_status miikv_evict(const miikv_view* view, const float* key_weights, uint64_t weight_stride, uint32_t batch,
+                         const uint32_t* d_lengths, uint32_t max_context, uint32_t sinks, uint32_t recent,
+                         uint32_t budget, const int32_t* dst_table, uint32_t dst_stride, int32_t* kept,
+                         uint32_t* d_new_lengths, float* weights_out, uint64_t weights_out_stride, void* stream);
+
 /* ---- export / import ----------------------------------------------------- */
 
 /* Copy tokens [t0, t0+count) of sequence `seq` out of the tiled cache into
@@ -457,6 +530,11 @@ miikv_status miikv_pool_prepare_append(miikv_pool* pool, int32_t* row, uint32_t 
  * those entries to -1 (a released row starts over as an empty row). */
 miikv_status miikv_pool_release(miikv_pool* pool, int32_t* row, uint32_t length,
                                 uint32_t page_tokens);
+/* After an eviction in place: drop one reference on each page of `row` that backs
+ * `length` tokens but none of the first new_length, and set those entries to -1.
+ * MIIKV_EINVAL, and nothing changed, for new_length > length or a bad row. */
+miikv_status miikv_pool_truncate(miikv_pool* pool, int32_t* row, uint32_t length, uint32_t new_length,
+                                 uint32_t page_tokens);
 
 /* Prefix fingerprint and match policy.  Restates ReusableContext
  * (include/miinfer/prefill_v2/reusable_context.hpp:17-129,

@@ -5,6 +5,13 @@ KV-cache / attention call surface; all compute runs in libmiikv.so (HIP,
 gfx950) and fails loudly when that library is missing.
 """
 from ._lib import MiikvError, lib  # noqa: F401
+from .bounded import (  # noqa: F401
+    evict,
+    scored_attention,
+    scored_workspace_bytes,
+    window_attention,
+    window_workspace_bytes,
+)
 from .kv import (  # noqa: F401
     DecodeWorkspace,
     advance_decode_state,
@@ -21,4 +28,5 @@ from .kv import (  # noqa: F401
 __all__ = [
     "MiikvError", "lib", "advance_decode_state", "KvCache", "DecodeWorkspace", "decode_attention", "clone_state",
     "copy_segments", "make_decode_state", "make_prefill_state", "suffix_attention", "suffix_workspace_bytes",
+    "evict", "scored_attention", "scored_workspace_bytes", "window_attention", "window_workspace_bytes",
 ]

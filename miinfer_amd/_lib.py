@@ -116,6 +116,14 @@ SIGNATURES = {
     "miikv_pool_fork_n": (ctypes.c_int, [_P, _P, _U32, _U32, _U32, _P, _U32, _P, _P, _P, _P]),
     "miikv_pool_prepare_append": (ctypes.c_int, [_P, _P, _U32, _U32, _U32, _P, _P, _P]),
     "miikv_pool_release": (ctypes.c_int, [_P, _P, _U32, _U32]),
+    "miikv_pool_truncate": (ctypes.c_int, [_P, _P, _U32, _U32, _U32]),
+    "miikv_window_workspace_bytes": (_U64, [_VP, _U32, _U32, _U32, _U32, _U32, _U32]),
+    "miikv_decode_attn_window": (ctypes.c_int, [_VP, _P, _U32, _U32, ctypes.c_float, _U32, _U32, _P, _P, _U32, _U32,
+                                                 _U32, _P, _P, _P, _P, _U64, _P]),
+    "miikv_scored_workspace_bytes": (_U64, [_VP, _U32, _U32, _U32, _U32]),
+    "miikv_decode_attn_scored": (ctypes.c_int, [_VP, _P, _U32, _U32, ctypes.c_float, _U32, _U32, _P, _P, _U32, _P,
+                                                 _U64, _P, _P, _P, _P, _U64, _P]),
+    "miikv_evict": (ctypes.c_int, [_VP, _P, _U64, _U32, _P, _U32, _U32, _U32, _U32, _P, _U32, _P, _P, _P, _U64, _P]),
     "miikv_token_hash": (_U64, [_P, ctypes.c_size_t]),
     "miikv_prefix_create": (_P, [ctypes.c_char_p, ctypes.c_char_p]),
     "miikv_prefix_destroy": (None, [_P]),

@@ -1,0 +1,219 @@
+"""Attention over part of a cache, and caches that are made smaller.
+
+``window_attention`` is decode attention with a sliding window and the first tokens that
+stay visible, ``scored_attention`` decode attention that adds up the weight every key
+gets, ``evict`` keeps the keys with the largest weights and moves their rows together.
+Every call goes through libmiikv; there is no fallback path.  The reference has no
+counterpart: its attention layers keep and see the whole context.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from ._lib import call, lib
+from .kv import KvCache, _on_stream, _ptr, _stream
+
+_INDEX = (torch.int32, torch.uint32)
+
+
+def _on_device(dev: torch.device):
+    """The cache's device current for the launch, where it is not already."""
+    if dev.type != "cuda":
+        raise ValueError("the cache must live on a GPU")
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _check(cache: KvCache, stream, **tensors) -> None:
+    """Every tensor on the cache's device, contiguous; the stream on it too."""
+    dev = cache.k_codes.device
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.device != dev:
+            raise ValueError(f"{name} must live on the cache's device")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+    if stream is not None and stream.device != dev:
+        raise ValueError("stream must be one of the cache's device")
+
+
+def _u32_arg(name: str, x: int, least: int = 0) -> int:
+    if not least <= x <= 0x7FFFFFFF:
+        raise ValueError(f"{name} out of range")
+    return x
+
+
+def _part_shape(cache: KvCache, q: torch.Tensor):
+    if q.dim() not in (3, 4) or q.shape[-1] != cache.head_dim or q.dtype not in (torch.float16, torch.float32):
+        raise ValueError("q must be fp16/fp32 [batch, q_heads, head_dim] or [batch, tokens, q_heads, head_dim]")
+    return q.shape[0], q.shape[1] if q.dim() == 4 else 1, q.shape[-2]
+
+
+def _check_batch(cache: KvCache, batch: int) -> None:
+    if cache.paged and batch > cache.block_table.shape[0]:
+        raise ValueError("batch exceeds the block-table rows")
+
+
+def _check_part(cache, q, lengths, decode_state, gate, out, gated_out, stream, **more):
+    batch, tokens, q_heads = _part_shape(cache, q)
+    _check(cache, stream, q=q, lengths=lengths, decode_state=decode_state, gate=gate, out=out, gated_out=gated_out, **more)
+    _check_batch(cache, batch)
+    if lengths is not None and (lengths.numel() < batch or lengths.dtype not in _INDEX):
+        raise ValueError("lengths must be int32 with one entry per sequence")
+    if decode_state is not None and decode_state.numel() * decode_state.element_size() < 64:
+        raise ValueError("decode_state must be a 64-byte device buffer")
+    for t in (gate, out, gated_out):
+        if t is not None and (t.shape != q.shape or t.dtype != torch.float32):
+            raise ValueError("gate/out/gated_out must be fp32, of q's shape")
+    return batch, tokens, q_heads
+
+
+def _outputs(q, gate, out, gated_out):
+    if out is None and gate is None:
+        out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+    if gate is not None and gated_out is None:
+        gated_out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+    return out, gated_out
+
+
+def _workspace(need: int, q: torch.Tensor) -> torch.Tensor:
+    if need == 0:
+        raise ValueError("the sizes are not ones that this call serves")
+    return torch.empty(need, dtype=torch.uint8, device=q.device)
+
+
+def window_workspace_bytes(cache: KvCache, q_heads: int, batch: int, tokens: int, max_context: int, window: int,
+                           sinks: int = 0) -> int:
+    return int(lib().miikv_window_workspace_bytes(cache.view, q_heads, batch, tokens, max_context, window, sinks))
+
+
+def window_attention(cache: KvCache, q: torch.Tensor, scale: float | None = None, *, window: int, sinks: int = 0,
+                     lengths: torch.Tensor | None = None, decode_state: torch.Tensor | None = None,
+                     max_context: int | None = None, gate: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                     gated_out: torch.Tensor | None = None, workspace: torch.Tensor | None = None, stream=None):
+    """Decode attention with a sliding window: the token at position p sees the keys j <= p
+    with j > p - window (window 0: all of them) or j < sinks.
+
+    q: [batch, q_heads, head_dim], or [batch, tokens, q_heads, head_dim] for the last `tokens`
+    tokens of every sequence (their rows already appended), fp16 or fp32.  Context lengths,
+    the new tokens included, come from `lengths` (device [batch]) or `decode_state`
+    (position + 1).  `workspace`: a uint8 tensor of window_workspace_bytes() (allocated when
+    not given); calls that may overlap need their own.  Returns (out, gated_out), fp32 of q's
+    shape."""
+    batch, tokens, q_heads = _check_part(cache, q, lengths, decode_state, gate, out, gated_out, stream, workspace=workspace)
+    if max_context is None:
+        max_context = cache.capacity
+    _u32_arg("window", window)
+    _u32_arg("sinks", sinks)
+    _u32_arg("max_context", max_context, 1)
+    with _on_device(cache.k_codes.device):
+        if workspace is None or out is None:
+            with _on_stream(stream):
+                if workspace is None:
+                    workspace = _workspace(window_workspace_bytes(cache, q_heads, batch, tokens, max_context, window, sinks), q)
+                out, gated_out = _outputs(q, gate, out, gated_out)
+        call("miikv_decode_attn_window", cache.view, q.data_ptr(), 0 if q.dtype == torch.float16 else 1, q_heads,
+             1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale), batch, tokens, _ptr(lengths),
+             _ptr(decode_state), max_context, window, sinks, _ptr(out), _ptr(gate), _ptr(gated_out),
+             workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(stream))
+    return out, gated_out
+
+
+def scored_workspace_bytes(cache: KvCache, q_heads: int, batch: int, tokens: int, max_context: int) -> int:
+    return int(lib().miikv_scored_workspace_bytes(cache.view, q_heads, batch, tokens, max_context))
+
+
+def scored_attention(cache: KvCache, q: torch.Tensor, key_weights: torch.Tensor, scale: float | None = None, *,
+                     lengths: torch.Tensor | None = None, decode_state: torch.Tensor | None = None,
+                     max_context: int | None = None, gate: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                     gated_out: torch.Tensor | None = None, workspace: torch.Tensor | None = None, stream=None):
+    """Decode attention over the whole context that adds every key's probabilities, summed
+    over the call's tokens and the query heads of a kv head, to `key_weights` (fp32 [batch,
+    kv_heads, n], n >= max_context; zeros for keys not seen yet).  The last tokens of a
+    prompt (q with a token axis) give the weights a first eviction goes by.  Other arguments
+    as window_attention.  Returns (out, gated_out)."""
+    batch, tokens, q_heads = _check_part(cache, q, lengths, decode_state, gate, out, gated_out, stream, workspace=workspace,
+                                         key_weights=key_weights)
+    if max_context is None:
+        max_context = cache.capacity
+    _u32_arg("max_context", max_context, 1)
+    _check_weights("key_weights", key_weights, batch, cache.kv_heads, max_context)
+    with _on_device(cache.k_codes.device):
+        if workspace is None or out is None:
+            with _on_stream(stream):
+                if workspace is None:
+                    workspace = _workspace(scored_workspace_bytes(cache, q_heads, batch, tokens, max_context), q)
+                out, gated_out = _outputs(q, gate, out, gated_out)
+        call("miikv_decode_attn_scored", cache.view, q.data_ptr(), 0 if q.dtype == torch.float16 else 1, q_heads,
+             1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale), batch, tokens, _ptr(lengths),
+             _ptr(decode_state), max_context, key_weights.data_ptr(), key_weights.shape[2], _ptr(out), _ptr(gate),
+             _ptr(gated_out), workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(stream))
+    return out, gated_out
+
+
+def _check_weights(name, w, batch, kv_heads, least):
+    if w.dtype != torch.float32 or w.dim() != 3 or w.shape[0] < batch or w.shape[1] != kv_heads or w.shape[2] < least:
+        raise ValueError(f"{name} must be fp32 [batch, kv_heads, >= {least}]")
+
+
+def evict(cache: KvCache, key_weights: torch.Tensor, lengths: torch.Tensor, *, budget: int, sinks: int = 0, recent: int = 0,
+          max_context: int | None = None, dst_table: torch.Tensor | None = None, kept: torch.Tensor | None = None,
+          new_lengths: torch.Tensor | None = None, weights_out: torch.Tensor | None = None, stream=None):
+    """Cut every sequence longer than `budget` down to it: per kv head the first `sinks` keys
+    stay, the last `recent`, and of those between the ones with the largest `key_weights`
+    ([batch, kv_heads, n], n >= max_context; of equal ones the first).  Their rows move, in order, to
+    positions 0, 1, ...: within the sequence's own pages, which nothing else may share then
+    (``PagePool.truncate`` gives the free ones back), or to the pages of `dst_table` (int32
+    [batch, pages], pages that the batch does not use; ``cache.set_block_table`` with it
+    afterwards).  `weights_out` (None: not kept) receives the kept keys' weights and may be
+    `key_weights`; `new_lengths` may be `lengths`.
+
+    A kept key keeps the rotation of its old position, so rows appended later have to come
+    rotated by theirs.  Returns (kept, new_lengths): the positions that stayed, int32 [batch,
+    kv_heads, budget], -1 past the new length, and min(length, budget)."""
+    dev = cache.k_codes.device
+    batch = key_weights.shape[0] if key_weights.dim() == 3 else 0
+    if lengths.dtype not in _INDEX or lengths.dim() != 1 or lengths.shape[0] != batch:
+        raise ValueError("lengths must be int32 [batch], with key_weights [batch, kv_heads, n]")
+    if max_context is None:
+        max_context = min(cache.capacity, key_weights.shape[2])
+    _u32_arg("max_context", max_context, 1)
+    _u32_arg("budget", budget, 1)
+    _u32_arg("sinks", sinks)
+    _u32_arg("recent", recent)
+    if sinks + recent > budget:
+        raise ValueError("sinks + recent exceed the budget")
+    _check_weights("key_weights", key_weights, batch, cache.kv_heads, max_context)
+    _check_batch(cache, batch)
+    _check(cache, stream, key_weights=key_weights, lengths=lengths, dst_table=dst_table, kept=kept, new_lengths=new_lengths,
+           weights_out=weights_out)
+    most = min(budget, max_context)
+    if weights_out is not None:
+        _check_weights("weights_out", weights_out, batch, cache.kv_heads, most)
+        if weights_out.shape[0] != batch:
+            raise ValueError("weights_out must have a row per sequence")
+    if kept is not None and (kept.dtype != torch.int32 or tuple(kept.shape) != (batch, cache.kv_heads, budget)):
+        raise ValueError("kept must be int32 [batch, kv_heads, budget]")
+    if new_lengths is not None and (new_lengths.dtype not in _INDEX or tuple(new_lengths.shape) != (batch,)):
+        raise ValueError("new_lengths must be int32 [batch]")
+    if dst_table is not None and (not cache.paged or dst_table.dtype != torch.int32 or dst_table.dim() != 2 or
+                                  dst_table.shape[0] < batch or dst_table.shape[1] * cache.page_tokens < most):
+        raise ValueError("dst_table must be int32 [batch, pages for the budget], of a paged cache")
+    with _on_device(dev):
+        if kept is None or new_lengths is None:
+            with _on_stream(stream):
+                if kept is None:
+                    kept = torch.empty((batch, cache.kv_heads, budget), dtype=torch.int32, device=dev)
+                if new_lengths is None:
+                    new_lengths = torch.empty((batch,), dtype=torch.int32, device=dev)
+        call("miikv_evict", cache.view, key_weights.data_ptr(), key_weights.shape[2], batch, lengths.data_ptr(), max_context,
+             sinks, recent, budget, _ptr(dst_table), 0 if dst_table is None else dst_table.shape[1], kept.data_ptr(),
+             new_lengths.data_ptr(), _ptr(weights_out), 0 if weights_out is None else weights_out.shape[2], _stream(stream))
+    return kept, new_lengths

@@ -20,6 +20,8 @@ SOURCES = [
     "miikv_cache.hip",
     "miikv_decode.hip",
     "miikv_suffix.hip",
+    "miikv_window.hip",
+    "miikv_evict.hip",
     "miikv_host.cpp",
     "miikv_session.cpp",
 ]

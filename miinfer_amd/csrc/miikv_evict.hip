@@ -1,0 +1,371 @@
+// Eviction: of every (sequence, kv head) the keys with the largest accumulated weight stay,
+// and their rows move together (gfx950).
+//
+// With L keys, a budget of n and L > n: the first `sinks` and the last `recent` keys stay,
+// and of those between the n - sinks - recent with the largest weights; of equal weights
+// the first ones.  Kept key i of the ascending list moves to position i.
+//
+// select_kernel finds the list: the weight that is just kept by a radix select over the
+// weights' ordered bits (four digits of 8 bits, counts in LDS), then each wave's place in
+// the list from counts of its own stretch of keys.  It also moves the weights.
+// move_kernel moves the rows: codes are copied as they are, nothing is quantised again.
+//
+// In place, position i's source is at or behind i, so rows that go forward in order never
+// overwrite one that is still to move: a workgroup owns a slice of every row (some bytes of
+// each token, which no other workgroup touches), reads kMoveTokens tokens, waits until all of
+// them have arrived, and writes them.  To other pages every tile is independent.
+//
+// Bound: the cache's lines that hold a kept row.  A K line of 128 bytes holds 8 tokens'
+// runs of 16 bytes and a V line 4 dims of 32 tokens, so where one key in eight stays nearly
+// all lines of the old context are read.
+#include "miikv_part.hpp"
+
+#include <type_traits>
+
+namespace miikv {
+namespace {
+
+constexpr uint32_t kSelectThreads = 1024;
+constexpr uint32_t kSelectWaves = kSelectThreads / 64;
+constexpr uint32_t kCopies = 16;    // histograms, one per lane % 16: weights share their top digits
+constexpr uint32_t kMoveTokens = 256;     // destination tokens moved at a time
+
+struct EvictArgs {
+    Geo g;
+    const int32_t* dst_table;  // null: in place
+    uint32_t dst_stride;
+    const float* weights;
+    uint64_t weight_stride;
+    float* weights_out;  // nullable
+    uint64_t weight_out_stride;
+    const uint32_t* lengths;
+    uint32_t* new_lengths;
+    int32_t* kept;
+    uint32_t batch;
+    uint32_t max_context;
+    uint32_t sinks, recent, budget;
+};
+
+__device__ __forceinline__ uint32_t evict_length(const EvictArgs& a, uint32_t b) { return min(a.lengths[b], a.max_context); }
+
+// Weights in the order of unsigned numbers; a NaN counts as less than any number.
+__device__ __forceinline__ uint32_t ordered(float w) {
+    if (w != w) return 0u;
+    const uint32_t u = __float_as_uint(w == 0.0f ? 0.0f : w);  // -0 equals 0
+    return (u & 0x80000000u) != 0 ? ~u : u | 0x80000000u;
+}
+
+__global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictArgs a) {
+    const uint32_t h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t L = evict_length(a, b), n = a.budget;
+    const size_t row = static_cast<size_t>(b) * a.g.kv_heads + h;
+    const float* w = a.weights + row * a.weight_stride;
+    int32_t* kept = a.kept + row * n;
+    const uint32_t left = min(L, n);  // keys that stay
+    __shared__ uint32_t s_hist[kCopies][256];
+    __shared__ uint32_t s_digit, s_need;
+    __shared__ uint32_t s_gt[kSelectWaves], s_eq[kSelectWaves];
+    if (L <= n) {
+        for (uint32_t i = tid; i < n; i += kSelectThreads) kept[i] = i < L ? static_cast<int32_t>(i) : -1;
+    } else {
+        const uint32_t lo = a.sinks, hi = L - a.recent, need = n - a.sinks - a.recent;
+        for (uint32_t i = tid; i < a.sinks; i += kSelectThreads) kept[i] = static_cast<int32_t>(i);
+        for (uint32_t i = tid; i < a.recent; i += kSelectThreads) kept[n - a.recent + i] = static_cast<int32_t>(hi + i);
+        if (need != 0) {  // and then hi - lo > need
+            uint32_t prefix = 0, mask = 0, k = need;
+            for (int shift = 24; shift >= 0; shift -= 8) {
+                for (uint32_t i = tid; i < kCopies * 256; i += kSelectThreads) (&s_hist[0][0])[i] = 0;
+                __syncthreads();
+                for (uint32_t i = lo + tid; i < hi; i += kSelectThreads) {
+                    const uint32_t u = ordered(w[i]);
+                    if ((u & mask) == prefix) atomicAdd(&s_hist[lane % kCopies][(u >> shift) & 255u], 1u);
+                }
+                __syncthreads();
+                if (tid < 256) {
+                    uint32_t sum = 0;
+#pragma unroll
+                    for (uint32_t c = 0; c < kCopies; ++c) sum += s_hist[c][tid];
+                    s_hist[0][tid] = sum;
+                }
+                __syncthreads();
+                if (wave == 0) {  // lane l: digits 255 - 4l down to 252 - 4l
+                    uint32_t c[4], sum = 0;
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) sum += c[j] = s_hist[0][255 - 4 * lane - j];
+                    uint32_t incl = sum;
+#pragma unroll
+                    for (uint32_t off = 1; off < 64; off <<= 1) {
+                        const uint32_t up = __shfl_up(incl, off, 64);
+                        if (lane >= off) incl += up;
+                    }
+                    uint32_t above = incl - sum;
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        if (above < k && k <= above + c[j]) {  // exactly one lane and digit
+                            s_digit = 255 - 4 * lane - j;
+                            s_need = k - above;
+                        }
+                        above += c[j];
+                    }
+                }
+                __syncthreads();
+                prefix |= s_digit << shift;
+                mask |= 255u << shift;
+                k = s_need;
+            }
+            // Keys above `prefix` stay, and the first k of those equal to it.
+            const uint32_t seg = ((hi - lo + kSelectWaves - 1) / kSelectWaves + 63) / 64 * 64;
+            const uint32_t from = min(lo + wave * seg, hi), to = min(from + seg, hi);
+            uint32_t gt = 0, eq = 0;
+            for (uint32_t i = from; i < to; i += 64) {
+                const uint32_t u = i + lane < to ? ordered(w[i + lane]) : 0u;
+                gt += static_cast<uint32_t>(__popcll(__ballot(i + lane < to && u > prefix)));
+                eq += static_cast<uint32_t>(__popcll(__ballot(i + lane < to && u == prefix)));
+            }
+            if (lane == 0) {
+                s_gt[wave] = gt;
+                s_eq[wave] = eq;
+            }
+            __syncthreads();
+            uint32_t gt0 = 0, eq0 = 0;
+            for (uint32_t x = 0; x < wave; ++x) {
+                gt0 += s_gt[x];
+                eq0 += s_eq[x];
+            }
+            uint32_t at = lo + gt0 + min(eq0, k);
+            const unsigned long long below = (1ull << lane) - 1ull;
+            for (uint32_t i = from; i < to; i += 64) {
+                const bool live = i + lane < to;
+                const uint32_t u = live ? ordered(w[i + lane]) : 0u;
+                const bool same = live && u == prefix;
+                const unsigned long long eqs = __ballot(same);
+                const uint32_t rank = eq0 + static_cast<uint32_t>(__popcll(eqs & below));
+                const bool keep = live && (u > prefix || (same && rank < k));
+                const unsigned long long keeps = __ballot(keep);
+                if (keep) kept[at + static_cast<uint32_t>(__popcll(keeps & below))] = static_cast<int32_t>(i + lane);
+                at += static_cast<uint32_t>(__popcll(keeps));
+                eq0 += static_cast<uint32_t>(__popcll(eqs));
+            }
+        }
+    }
+    if (a.weights_out == nullptr) return;
+    float* out = a.weights_out + row * a.weight_out_stride;
+    const bool same_row = out == w;
+    if (same_row && L <= n) return;
+    __syncthreads();  // the list is whole, and the weights have been read
+    for (uint32_t i0 = 0; i0 < left; i0 += kSelectThreads) {
+        const uint32_t i = i0 + tid;
+        const float x = i < left ? w[kept[i]] : 0.0f;
+        if (same_row) {
+            wait_vmem();
+            __syncthreads();
+        }
+        if (i < left) out[i] = x;
+    }
+    // in place: what stood behind the keys that stay is no weight of the keys to come
+    if (same_row)
+        for (uint32_t i = left + tid; i < L; i += kSelectThreads) {
+            out[i] = 0.0f;
+        }
+}
+
+typedef unsigned int u4v __attribute__((ext_vector_type(4)));
+
+// Row (page * kv_heads + head) * page_tokens + slot of position `pos`.
+__device__ __forceinline__ uint32_t row_of(const Geo& g, const int32_t* table, uint32_t pos, uint32_t h) {
+    uint32_t page = 0, tp = pos;
+    if (table != nullptr) {
+        const uint32_t e = pos / g.page_tokens;
+        tp = pos - e * g.page_tokens;
+        page = min(static_cast<uint32_t>(table[e]), g.num_pages - 1);
+    }
+    return (page * g.kv_heads + h) * g.page_tokens + tp;
+}
+
+// Roles of a (sequence, kv head)'s workgroups: D / 32 slices of K (4 runs of 8 + 8 dims),
+// D / 32 of V (32 dims), one of the scales.
+template <uint32_t D, bool KF16, bool VF16, bool INPLACE>
+__global__ void __launch_bounds__(kMoveTokens) move_kernel(EvictArgs a) {
+    constexpr uint32_t NB = D / 32;
+    constexpr uint32_t kRoles = 2 * (D / 64) + NB + 1;
+    constexpr uint32_t KE = KF16 ? 2 : 1;
+    const uint32_t role = blockIdx.x % kRoles, tile = blockIdx.x / kRoles;
+    const uint32_t h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+    const uint32_t left = min(evict_length(a, b), a.budget);
+    if (!INPLACE && tile == 0 && role == 0 && h == 0 && tid == 0) a.new_lengths[b] = left;
+    const int32_t* kept = a.kept + (static_cast<size_t>(b) * a.g.kv_heads + h) * a.budget;
+    const int32_t* src_table = a.g.layout == MIIKV_LAYOUT_PAGED ? a.g.table + static_cast<size_t>(b) * a.g.table_stride : nullptr;
+    const int32_t* dst_table = INPLACE ? src_table : a.dst_table + static_cast<size_t>(b) * a.dst_stride;
+    // Two buffers: a wave may write the next tile's rows while another still stores this one's.
+    __shared__ uint32_t s_rows[2][2][kMoveTokens];
+    uint32_t turn = 0;
+    for (uint32_t t0 = tile * kMoveTokens; t0 < left; t0 += kMoveTokens, turn ^= 1) {
+        uint32_t *s_src = s_rows[turn][0], *s_dst = s_rows[turn][1];
+        const uint32_t i = t0 + tid;
+        bool moves = false;
+        if (i < left) {
+            const uint32_t from = static_cast<uint32_t>(kept[i]);
+            moves = !INPLACE || from != i;
+            s_src[tid] = row_of(a.g, src_table, from, h);
+            s_dst[tid] = row_of(a.g, dst_table, i, h);
+        }
+        if (!__syncthreads_or(moves) && INPLACE) continue;  // nothing of this tile moves
+        const uint32_t count = min(kMoveTokens, left - t0);
+        if (role < 2 * (D / 64)) {
+            // token tid's runs of 16 * KE bytes: chunk c = role / 2, g = 2 (role % 2) + 0, 1
+            u4v r[2][KE];
+            const size_t off = static_cast<size_t>(role / 2) * 1024 + (role % 2) * 512;
+            if (tid < count) {
+                const size_t row = s_src[tid];
+                const int8_t* p = a.g.k_codes + KE * ((row & ~size_t{15}) * D + off + (row & 15) * 16);
+#pragma unroll
+                for (uint32_t u = 0; u < 2; ++u)
+#pragma unroll
+                    for (uint32_t e = 0; e < KE; ++e) r[u][e] = *reinterpret_cast<const u4v*>(p + KE * u * 256 + 16 * e);
+            }
+            if constexpr (INPLACE) {
+                wait_vmem();
+                __syncthreads();
+            }
+            if (tid < count) {
+                const size_t row = s_dst[tid];
+                int8_t* p = a.g.k_codes + KE * ((row & ~size_t{15}) * D + off + (row & 15) * 16);
+#pragma unroll
+                for (uint32_t u = 0; u < 2; ++u)
+#pragma unroll
+                    for (uint32_t e = 0; e < KE; ++e) *reinterpret_cast<u4v*>(p + KE * u * 256 + 16 * e) = r[u][e];
+            }
+        } else if (role < 2 * (D / 64) + NB) {
+            // 8 groups of 32 tokens x 32 dims x 4 units of 8 tokens (16 (x / 4) + 4 G + x % 4)
+            using Elem = typename std::conditional<VF16, uint16_t, uint8_t>::type;
+            constexpr uint32_t kPer = VF16 ? 2 : 4;  // elements of a 32-bit word
+            const uint32_t d0 = (role - 2 * (D / 64)) * 32;
+            const Elem* v = reinterpret_cast<const Elem*>(a.g.v_codes);
+            constexpr uint32_t kUnits = 32 / 8;  // per thread
+            uint32_t r[kUnits][8 / kPer];
+#pragma unroll
+            for (uint32_t j = 0; j < kUnits; ++j) {
+                const uint32_t x = j * kMoveTokens + tid, G = x & 3, d = d0 + ((x >> 2) & 31), H = x >> 7;
+#pragma unroll
+                for (uint32_t k = 0; k < 8; ++k) {
+                    const uint32_t t = min(32 * H + 16 * (k / 4) + 4 * G + k % 4, count - 1);
+                    const size_t row = s_src[t];
+                    const uint32_t s = static_cast<uint32_t>(row & 31);
+                    const uint32_t e = v[(row & ~size_t{31}) * D + d * 32 + ((s >> 2) & 3) * 8 + (s >> 4) * 4 + (s & 3)];
+                    if (k % kPer == 0) r[j][k / kPer] = e;
+                    else r[j][k / kPer] |= e << (32 / kPer * (k % kPer));
+                }
+            }
+            if constexpr (INPLACE) {
+                wait_vmem();
+                __syncthreads();
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < kUnits; ++j) {
+                const uint32_t x = j * kMoveTokens + tid, G = x & 3, d = d0 + ((x >> 2) & 31), H = x >> 7;
+                if (32 * H + 4 * G >= count) continue;
+                const size_t row = s_dst[32 * H];  // a group's rows are consecutive
+                Elem* to = reinterpret_cast<Elem*>(a.g.v_codes) + row * D + d * 32 + G * 8;
+                if (32 * H + 16 + 4 * G + 3 < count) {
+                    uint32_t* word = reinterpret_cast<uint32_t*>(to);
+#pragma unroll
+                    for (uint32_t k = 0; k < 8 / kPer; ++k) word[k] = r[j][k];
+                } else {  // the last group: what is behind the kept rows stays as it was
+#pragma unroll
+                    for (uint32_t k = 0; k < 8; ++k)
+                        if (32 * H + 16 * (k / 4) + 4 * G + k % 4 < count) to[k] = static_cast<Elem>(r[j][k / kPer] >> (32 / kPer * (k % kPer)));
+                }
+            }
+        } else {
+            using ScaleRow = typename std::conditional<NB == 4, uint2, uint4>::type;
+            ScaleRow ks{}, vs{};
+            if (tid < count) {
+                if constexpr (!KF16) ks = *reinterpret_cast<const ScaleRow*>(a.g.k_scales + static_cast<size_t>(s_src[tid]) * NB);
+                if constexpr (!VF16) vs = *reinterpret_cast<const ScaleRow*>(a.g.v_scales + static_cast<size_t>(s_src[tid]) * NB);
+            }
+            if constexpr (INPLACE) {
+                wait_vmem();
+                __syncthreads();
+            }
+            if (tid < count) {
+                if constexpr (!KF16) *reinterpret_cast<ScaleRow*>(a.g.k_scales + static_cast<size_t>(s_dst[tid]) * NB) = ks;
+                if constexpr (!VF16) *reinterpret_cast<ScaleRow*>(a.g.v_scales + static_cast<size_t>(s_dst[tid]) * NB) = vs;
+            }
+        }
+        if constexpr (!INPLACE) break;
+    }
+    // `new_lengths` may be `lengths`: min(length, budget) is the same of the old and of the new one
+    if (INPLACE && role == 0 && h == 0 && tid == 0) a.new_lengths[b] = left;
+}
+
+int evict_sizes(const miikv_view* v, uint32_t batch, uint32_t max_context, uint32_t budget) {
+    const int st = validate_view(v);
+    if (st != MIIKV_OK) return st;
+    if (batch == 0 || batch > 65535u || v->kv_heads > 65535u || budget == 0 || budget > 0x7fffffffu) return MIIKV_EINVAL;
+    if (max_context == 0 || max_context > view_seq_capacity(v) || max_context > 0x7fffffffu) return MIIKV_EINVAL;
+    if (v->layout == MIIKV_LAYOUT_CONTIGUOUS && batch != 1) return MIIKV_EINVAL;
+    return MIIKV_OK;
+}
+
+template <uint32_t D>
+void launch_move(const EvictArgs& a, bool kf, bool vf, hipStream_t s) {
+    const uint32_t most = a.max_context < a.budget ? a.max_context : a.budget;
+    const uint32_t tiles = a.dst_table != nullptr ? (most + kMoveTokens - 1) / kMoveTokens : 1u;
+    const dim3 grid((2 * (D / 64) + D / 32 + 1) * tiles, a.g.kv_heads, a.batch);
+    const auto go = [&](auto k, auto v, auto in) {
+        hipLaunchKernelGGL((move_kernel<D, decltype(k)::value, decltype(v)::value, decltype(in)::value>), grid, dim3(kMoveTokens), 0, s, a);
+    };
+    const auto with_in = [&](auto k, auto v) { a.dst_table == nullptr ? go(k, v, std::true_type{}) : go(k, v, std::false_type{}); };
+    const auto with_v = [&](auto k) { vf ? with_in(k, std::true_type{}) : with_in(k, std::false_type{}); };
+    kf ? with_v(std::true_type{}) : with_v(std::false_type{});
+}
+
+}  // namespace
+}  // namespace miikv
+
+using namespace miikv;
+
+extern "C" miikv_status miikv_evict(const miikv_view* view, const float* key_weights, uint64_t weight_stride,
+                                    uint32_t batch, const uint32_t* d_lengths, uint32_t max_context, uint32_t sinks,
+                                    uint32_t recent, uint32_t budget, const int32_t* dst_table, uint32_t dst_stride,
+                                    int32_t* kept, uint32_t* d_new_lengths, float* weights_out,
+                                    uint64_t weights_out_stride, void* stream) {
+    const int st = evict_sizes(view, batch, max_context, budget);
+    if (st != MIIKV_OK) return st;
+    if (key_weights == nullptr || weight_stride < max_context || d_lengths == nullptr || kept == nullptr ||
+        d_new_lengths == nullptr)
+        return MIIKV_EINVAL;
+    if (static_cast<uint64_t>(sinks) + recent > budget) return MIIKV_EINVAL;
+    const uint32_t most = max_context < budget ? max_context : budget;
+    if (weights_out == key_weights ? weights_out_stride != weight_stride : weights_out != nullptr && weights_out_stride < most)
+        return MIIKV_EINVAL;
+    if (dst_table != nullptr &&
+        (view->layout != MIIKV_LAYOUT_PAGED || static_cast<uint64_t>(dst_stride) * view->page_tokens < most))
+        return MIIKV_EINVAL;
+    if (!aligned16(view->k_codes) || !aligned16(view->v_codes) || !aligned16(view->k_scales) || !aligned16(view->v_scales))
+        return MIIKV_EINVAL;
+    const uint64_t tiles = (static_cast<uint64_t>(most) + kMoveTokens - 1) / kMoveTokens;
+    if (tiles * (view->head_dim / 16 + 1) > 0x7fffffffu) return MIIKV_EINVAL;
+    EvictArgs a{};
+    a.g = make_geo(*view);
+    a.dst_table = dst_table;
+    a.dst_stride = dst_stride;
+    a.weights = key_weights;
+    a.weight_stride = weight_stride;
+    a.weights_out = weights_out;
+    a.weight_out_stride = weights_out_stride;
+    a.lengths = d_lengths;
+    a.new_lengths = d_new_lengths;
+    a.kept = kept;
+    a.batch = batch;
+    a.max_context = max_context;
+    a.sinks = sinks;
+    a.recent = recent;
+    a.budget = budget;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(select_kernel, dim3(view->kv_heads, batch), dim3(kSelectThreads), 0, s, a);
+    const bool kf = mode_k_f16(view->quant_mode), vf = mode_v_f16(view->quant_mode);
+    if (view->head_dim == 128) launch_move<128>(a, kf, vf, s);
+    else launch_move<256>(a, kf, vf, s);
+    return hip_status(hipGetLastError());
+}

@@ -186,6 +186,19 @@ extern "C" miikv_status miikv_pool_release(miikv_pool* p, int32_t* row, uint32_t
     return MIIKV_OK;
 }
 
+extern "C" miikv_status miikv_pool_truncate(miikv_pool* p, int32_t* row, uint32_t length, uint32_t new_length,
+                                            uint32_t page_tokens) {
+    if (p == nullptr || page_tokens == 0 || new_length > length || (length > 0 && row == nullptr)) return MIIKV_EINVAL;
+    const uint32_t from = pages_for(new_length, page_tokens), np = pages_for(length, page_tokens);
+    for (uint32_t i = 0; i < np; ++i)
+        if (!valid_page(p, row[i]) || p->refs[static_cast<size_t>(row[i])] == 0) return MIIKV_EINVAL;
+    for (uint32_t i = from; i < np; ++i) {
+        miikv_pool_unref(p, row[i]);
+        row[i] = -1;
+    }
+    return MIIKV_OK;
+}
+
 // ---------------------------------------------------------------------------
 // Prefix fingerprint and match policy: restates ReusableContext
 // (include/miinfer/prefill_v2/reusable_context.hpp:17-129,

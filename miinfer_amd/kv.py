@@ -87,6 +87,43 @@ class KvCache:
                     page_tokens: int = 256, device="cuda", quant_mode: int = _lib.KV_Q8_Q8) -> "KvCache":
         return cls(kv_heads, head_dim, page_tokens, num_pages, block_table, device, quant_mode)
 
+    @classmethod
+    def from_planes(cls, kv_heads: int, head_dim: int, k_codes: torch.Tensor, v_codes: torch.Tensor,
+                    k_scales: torch.Tensor | None = None, v_scales: torch.Tensor | None = None, *, page_tokens: int,
+                    block_table: torch.Tensor | None = None) -> "KvCache":
+        """A cache over planes that the caller holds, in the tiled order of include/miikv.h
+        (nothing is copied): int8 codes with int16 (fp16 bits) scales, or fp16 rows without.
+        Contiguous (`page_tokens` the capacity) without a block table, paged with one."""
+        if page_tokens <= 0 or page_tokens % 64 != 0:
+            raise ValueError("page_tokens must be a multiple of 64")
+        per = kv_heads * page_tokens
+        pages = k_codes.numel() // (per * head_dim)
+        for codes, scales in ((k_codes, k_scales), (v_codes, v_scales)):
+            if codes.dtype not in (torch.int8, torch.float16) or codes.numel() != pages * per * head_dim:
+                raise ValueError("codes must be int8 or fp16, whole pages of both planes")
+            if (scales is None) != (codes.dtype == torch.float16):
+                raise ValueError("int8 codes go with scales, fp16 rows without")
+            if scales is not None and (scales.dtype not in (torch.int16, torch.float16) or
+                                       scales.numel() != pages * per * (head_dim // QBLOCK)):
+                raise ValueError("scales must be int16 or fp16, one per 32 codes")
+            for t in (codes, scales):
+                if t is not None and (t.device != k_codes.device or not t.is_contiguous()):
+                    raise ValueError("planes must be contiguous, on one device")
+        if pages == 0 or (block_table is None and pages != 1):
+            raise ValueError("a contiguous cache is one page")
+        if block_table is not None and block_table.device != k_codes.device:
+            raise ValueError("the block table must live on the planes' device")
+        c = cls.__new__(cls)
+        c.kv_heads, c.head_dim, c.page_tokens, c.num_pages = kv_heads, head_dim, page_tokens, pages
+        c.paged, c.block_table = block_table is not None, block_table
+        c.k_f16, c.v_f16 = k_scales is None, v_scales is None
+        c.quant_mode = {(True, True): _lib.KV_FP16_FP16, (False, True): _lib.KV_Q8_FP16, (True, False): _lib.KV_FP16_Q8,
+                        (False, False): _lib.KV_Q8_Q8}[c.k_f16, c.v_f16]
+        c.k_codes, c.v_codes, c.k_scales, c.v_scales = k_codes, v_codes, k_scales, v_scales
+        c._view = MiikvView()
+        c._refresh_view()
+        return c
+
     def _refresh_view(self) -> None:
         v = self._view
         v.k_codes = self.k_codes.data_ptr()

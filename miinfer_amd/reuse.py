@@ -100,6 +100,14 @@ class PagePool:
              _i32p(src), _i32p(dst), ctypes.byref(n))
         return [(int(src[0]), int(dst[0]))] if n.value else []
 
+    def truncate(self, row: np.ndarray, length: int, new_length: int, page_tokens: int) -> None:
+        """After an eviction in place: drop the row's references on the pages that back
+        none of the first `new_length` tokens; their entries become -1 (in place)."""
+        work = np.ascontiguousarray(row, np.int32)
+        call("miikv_pool_truncate", self._h, _i32p(work), length, new_length, page_tokens)
+        if work is not row:
+            row[...] = work
+
     def release(self, row: np.ndarray, length: int, page_tokens: int) -> None:
         """Drop the row's page references; its entries become -1 (in place)."""
         work = np.ascontiguousarray(row, np.int32)
