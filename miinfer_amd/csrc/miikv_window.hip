@@ -14,9 +14,10 @@
 // The results are fp32 and hold fp32's precision: the codes enter the MFMAs as exact fp16
 // integers, K's block scales are applied to fp32 sums, an fp32 query as hi + lo fp16 parts,
 // and the probabilities (times V's block scale) as hi + lo fp16 parts too, 22 bits in all.
-// P's parts are kept 2^kPShift above the true value, so that what a probability of 2^-20
-// adds is still no fp16 denormal; p <= 1 and a scale is at most 65504 / 127, so the
-// product stays below 65504.
+// P enters 2^shift above its value, so that both parts of a probability of 2^-20 stay clear
+// of fp16's denormals: p <= 1 is multiplied by V's block scale, so shift is what the largest
+// scale so far leaves below 2^15 (scales of 0.02: shift 20; with 6, outputs were 3.6e-6
+// off instead of 4e-7).
 //
 // Work: the visible 32-key steps of all sequences are cut into runs of 4 * cpw steps, one
 // workgroup (of four waves) each.  cpw is chosen on the device from the lengths, so that
@@ -32,7 +33,8 @@ namespace miikv {
 namespace {
 
 constexpr uint32_t kWaves = 4;            // waves per workgroup
-constexpr float kPShift = 6.0f;           // log2 of what P's parts are scaled by
+constexpr int kMinShift = -1;             // 2^-1 * 65504 < 2^15
+constexpr int kMaxShift = 24;
 constexpr uint32_t kTargetWgs = 512;      // two workgroups per CU
 constexpr uint32_t kWeightKeys = 256;     // keys per workgroup of the weights pass
 
@@ -52,7 +54,9 @@ struct PartArgs {
     uint32_t sinks;
     uint32_t batch;
     uint32_t target_wgs;
-    float* part;     // a record per run: o [cols][D], m [cols], l [cols], padded to 4
+    uint32_t* runs;  // [batch][kv_heads][2]: first record and records of a pair that has any
+    float* part;     // a record per run: o [cols][D], r [cols], l [cols], padded to 4, where
+                     // o = sum of 2^(s - r) v and l = sum of 2^(s - r)
     float* logits;   // SCORED: scores in log2 units [batch][kv_heads][cols][logit_keys]
     uint32_t logit_keys;
     float* weights;  // SCORED: [batch][kv_heads][weight_stride]
@@ -78,8 +82,6 @@ struct Run {
     uint32_t b, h;
     uint32_t split;  // number of the run among (b, h)'s
     uint32_t runs;   // of (b, h)
-    uint32_t first;  // record of (b, h)'s first run
-    uint32_t cpw;
     bool live;
 };
 
@@ -99,8 +101,18 @@ __device__ __forceinline__ uint32_t steps_per_wave(const PartArgs& a) {
 __device__ __forceinline__ Run find_run(const PartArgs& a, uint32_t w) {
     const uint32_t lane = threadIdx.x & 63;
     Run r{};
-    r.cpw = steps_per_wave(a);
-    const uint32_t quota = kWaves * r.cpw;
+    if (a.batch == 1) {
+        const uint32_t n = part_steps(a, 0);
+        const uint32_t quota = kWaves * max(1u, (n * a.g.kv_heads + a.target_wgs * kWaves - 1) / (a.target_wgs * kWaves));
+        r.runs = __builtin_amdgcn_readfirstlane((n + quota - 1) / quota);
+        r.live = w < r.runs * a.g.kv_heads;
+        if (r.live) {
+            r.h = w / r.runs;
+            r.split = w - r.h * r.runs;
+        }
+        return r;
+    }
+    const uint32_t quota = kWaves * steps_per_wave(a);
     uint32_t base = 0;
     for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
         const uint32_t n = b0 + lane < a.batch ? (part_steps(a, b0 + lane) + quota - 1) / quota : 0u;
@@ -115,14 +127,11 @@ __device__ __forceinline__ Run find_run(const PartArgs& a, uint32_t w) {
         const unsigned long long at = __ballot(w >= before && w < before + mine);
         if (at != 0) {
             const int src = __builtin_ctzll(at);
-            const uint32_t runs = __builtin_amdgcn_readfirstlane(__shfl(n, src, 64));
-            const uint32_t first = __builtin_amdgcn_readfirstlane(__shfl(before, src, 64));
-            const uint32_t x = w - first;
+            const uint32_t x = w - __builtin_amdgcn_readfirstlane(__shfl(before, src, 64));
+            r.runs = __builtin_amdgcn_readfirstlane(__shfl(n, src, 64));
             r.b = b0 + static_cast<uint32_t>(src);
-            r.h = x / runs;
-            r.split = x % runs;
-            r.runs = runs;
-            r.first = first + r.h * runs;
+            r.h = x / r.runs;
+            r.split = x - r.h * r.runs;
             r.live = true;
             return r;
         }
@@ -131,16 +140,11 @@ __device__ __forceinline__ Run find_run(const PartArgs& a, uint32_t w) {
     return r;
 }
 
-// Records of (b, h): the first and how many.
-__device__ __forceinline__ void find_records(const PartArgs& a, uint32_t b, uint32_t h, uint32_t& first, uint32_t& runs) {
-    const uint32_t lane = threadIdx.x & 63;
-    const uint32_t quota = kWaves * steps_per_wave(a);
-    uint32_t sum = 0;
-    for (uint32_t i = lane; i < b; i += 64) sum += (part_steps(a, i) + quota - 1) / quota;
-#pragma unroll
-    for (uint32_t off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off, 64);
-    runs = (part_steps(a, b) + quota - 1) / quota;
-    first = sum * a.g.kv_heads + h * runs;
+// Records of (b, h), which the first launch has noted for pairs that see any key.
+__device__ __forceinline__ void find_records(const PartArgs& a, uint32_t bh, uint32_t b, uint32_t& first, uint32_t& runs) {
+    const uint2 at = *reinterpret_cast<const uint2*>(a.runs + 2 * static_cast<size_t>(bh));
+    first = at.x;
+    runs = part_length(a, b) != 0 ? at.y : 0u;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -156,8 +160,15 @@ __device__ __forceinline__ uint2 stream8(const void* p) {
     return make_uint2(t.x, t.y);
 }
 
+// Waves per SIMD that an instance is compiled for.
+template <uint32_t D, bool QF32, bool KF16, bool VF16>
+constexpr uint32_t part_waves_per_eu() {
+    return D == 256 && (QF32 || KF16 || VF16) ? 1u : 2u;
+}
+
 template <uint32_t D, bool QF32, bool KF16, bool VF16, bool SCORED>
-__global__ void __launch_bounds__(64 * kWaves) part_kernel(PartArgs a) {
+__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(part_waves_per_eu<D, QF32, KF16, VF16>())))
+part_kernel(PartArgs a) {
     constexpr uint32_t NB = D / 32;  // q8_0 blocks per row
     constexpr uint32_t NC = D / 64;
     constexpr uint32_t NM = D / 16;  // 16-dim tiles of V
@@ -172,7 +183,12 @@ __global__ void __launch_bounds__(64 * kWaves) part_kernel(PartArgs a) {
     const Geo& geo = a.g;
     const uint32_t L = part_length(a, b);
     const Visible vis = visible_steps(L, a.tokens, a.window, a.sinks);
-    const uint32_t total = vis.steps();
+    // The pair's steps are cut evenly into its runs.
+    const uint32_t steps = vis.steps();
+    const uint32_t from = static_cast<uint32_t>(static_cast<uint64_t>(steps) * run.split / run.runs);
+    const uint32_t to = static_cast<uint32_t>(static_cast<uint64_t>(steps) * (run.split + 1) / run.runs);
+    if (run.split == 0 && threadIdx.x == 0)
+        *reinterpret_cast<uint2*>(a.runs + 2 * (static_cast<size_t>(b) * geo.kv_heads + h)) = make_uint2(blockIdx.x, run.runs);
 
     // Column n: token n / heads at position at_n (none: sees no key), query head n % heads.
     const bool col = n < a.cols;
@@ -204,13 +220,14 @@ __global__ void __launch_bounds__(64 * kWaves) part_kernel(PartArgs a) {
         }
     }
 
-    struct Step {
-        uint4 k[2][NC][KF16 ? 2 : 1];
-        typename std::conditional<VF16, uint4, uint2>::type v[NM];
-        ScaleVec ks, vs;
-    };
-    const uint32_t first = run.split * kWaves * run.cpw;
-    auto load_step = [&](uint32_t i, Step& st) __attribute__((always_inline)) {
+    // Registers of one step.  K's are loaded again for the next step as soon as the scores
+    // have read them, V's after the values: half a step is always in flight, and no second
+    // set of registers is held.
+    uint4 kreg[2][NC][KF16 ? 2 : 1];
+    typename std::conditional<VF16, uint4, uint2>::type vreg[NM];
+    ScaleVec ksc{}, vsc{};
+    constexpr uint32_t KE = KF16 ? 2 : 1, VE = VF16 ? 2 : 1;
+    auto row_at = [&](uint32_t i) __attribute__((always_inline)) {
         const uint32_t tok0 = vis.step(i) * kChunk;
         uint32_t page = 0, tp = tok0;
         if (geo.layout == MIIKV_LAYOUT_PAGED) {
@@ -219,48 +236,55 @@ __global__ void __launch_bounds__(64 * kWaves) part_kernel(PartArgs a) {
             page = min(static_cast<uint32_t>(scalar_load(geo.table + static_cast<size_t>(b) * geo.table_stride + e)),
                        geo.num_pages - 1);
         }
-        const size_t row = (static_cast<size_t>(page) * geo.kv_heads + h) * geo.page_tokens + tp;
-        constexpr uint32_t KE = KF16 ? 2 : 1, VE = VF16 ? 2 : 1;
+        return (static_cast<size_t>(page) * geo.kv_heads + h) * geo.page_tokens + tp;
+    };
+    auto load_k = [&](size_t row) __attribute__((always_inline)) {
         const int8_t* kb = geo.k_codes + row * (D * KE);
-        const int8_t* vb = geo.v_codes + row * (D * VE);
-        if constexpr (!KF16) st.ks = *reinterpret_cast<const ScaleVec*>(geo.k_scales + row * NB + lane * (NB / 2));
+        if constexpr (!KF16) ksc = *reinterpret_cast<const ScaleVec*>(geo.k_scales + row * NB + lane * (NB / 2));
 #pragma unroll
         for (uint32_t J = 0; J < 2; ++J)
 #pragma unroll
             for (uint32_t c = 0; c < NC; ++c)
 #pragma unroll
                 for (uint32_t e = 0; e < KE; ++e)
-                    st.k[J][c][e] = stream16(kb + KE * (J * 16 * D + c * 1024 + g4 * 256 + n * 16) + 16 * e);
-        if constexpr (!VF16) st.vs = *reinterpret_cast<const ScaleVec*>(geo.v_scales + row * NB + lane * (NB / 2));
+                    kreg[J][c][e] = stream16(kb + KE * (J * 16 * D + c * 1024 + g4 * 256 + n * 16) + 16 * e);
+    };
+    auto load_v = [&](size_t row) __attribute__((always_inline)) {
+        const int8_t* vb = geo.v_codes + row * (D * VE);
+        if constexpr (!VF16) vsc = *reinterpret_cast<const ScaleVec*>(geo.v_scales + row * NB + lane * (NB / 2));
 #pragma unroll
         for (uint32_t mt = 0; mt < NM; ++mt) {
-            if constexpr (VF16) st.v[mt] = stream16(vb + 2 * ((16 * mt + n) * 32 + g4 * 8));
-            else st.v[mt] = stream8(vb + (16 * mt + n) * 32 + g4 * 8);
+            if constexpr (VF16) vreg[mt] = stream16(vb + 2 * ((16 * mt + n) * 32 + g4 * 8));
+            else vreg[mt] = stream8(vb + (16 * mt + n) * 32 + g4 * 8);
         }
     };
 
-    float m_run = -INFINITY, l_run = 0.0f;
+    // p = 2^(s - ref); ref is `shift` below the column's running maximum.
+    float ref = -INFINITY, l_run = 0.0f;
+    int shift = VF16 ? 14 : kMaxShift;
+    bool fresh = true;  // no key seen by this wave yet
     float4v O[NM];
 #pragma unroll
     for (uint32_t mt = 0; mt < NM; ++mt) O[mt] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
     uint16_t* s_sc = reinterpret_cast<uint16_t*>(smem) + wave * (2 * kChunk * NB);
     const size_t pair = static_cast<size_t>(b) * geo.kv_heads + h;
 
-    auto compute = [&](uint32_t i, const Step& st) __attribute__((always_inline)) {
+    uint32_t i = from + wave;
+    size_t row = 0;
+    if (i < to) {
+        row = row_at(i);
+        load_k(row);
+        load_v(row);
+    }
+    for (; i < to; i += kWaves) {
         const uint32_t tok0 = vis.step(i) * kChunk;
-        asm volatile("" ::: "memory");  // the previous step's reads of the scales stay before it
+        const bool next = i + kWaves < to;
+        if (next) row = row_at(i + kWaves);
         // Every column sees every key of the step, or there is something to mask.
         const bool whole = tok0 + kChunk + a.tokens <= L + 1 &&
                            (a.window == 0 || tok0 + kChunk <= a.sinks || tok0 + a.window >= L);
-        if constexpr (!KF16) *reinterpret_cast<ScaleVec*>(s_sc + lane * (NB / 2)) = st.ks;
-        if constexpr (!VF16) {
-            ScaleVec x = st.vs;
-            if (!whole) {  // keys that no column sees may hold anything, non-finite scales too
-                const uint32_t t = tok0 + lane / 2;
-                if (t >= L || (t < vis.lo && t >= a.sinks)) x = ScaleVec{};
-            }
-            *reinterpret_cast<ScaleVec*>(s_sc + kChunk * NB + lane * (NB / 2)) = x;
-        }
+        asm volatile("" ::: "memory");  // the previous step's reads of the scales stay before it
+        if constexpr (!KF16) *reinterpret_cast<ScaleVec*>(s_sc + lane * (NB / 2)) = ksc;
         asm volatile("" ::: "memory");
         // Scores S^T[key][column], one MFMA per 32-value block and its scale in fp32.
         float s[2][4];
@@ -271,7 +295,7 @@ __global__ void __launch_bounds__(64 * kWaves) part_kernel(PartArgs a) {
                 float4v c = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (uint32_t blk = 0; blk < NB; ++blk) {
-                    const half8 k = __builtin_bit_cast(half8, st.k[J][blk / 2][KF16 ? blk % 2 : 0]);
+                    const half8 k = __builtin_bit_cast(half8, kreg[J][blk / 2][KF16 ? blk % 2 : 0]);
                     c = mfma_16x16x32(k, qf[blk], c);
                     if constexpr (QF32) c = mfma_16x16x32(k, ql[QF32 ? blk : 0], c);
                 }
@@ -285,7 +309,7 @@ __global__ void __launch_bounds__(64 * kWaves) part_kernel(PartArgs a) {
                 const uint16_t* sc = reinterpret_cast<const uint16_t*>(&w[0]);
 #pragma unroll
                 for (uint32_t blk = 0; blk < NB; ++blk) {
-                    const uint4 kw = st.k[J][blk / 2][0];
+                    const uint4 kw = kreg[J][blk / 2][0];
                     const half8 k = blk % 2 == 0 ? codes8_to_half8(kw.x, kw.y) : codes8_to_half8(kw.z, kw.w);
                     float4v c = mfma_16x16x32(k, qf[blk], float4v{0.0f, 0.0f, 0.0f, 0.0f});
                     if constexpr (QF32) c = mfma_16x16x32(k, ql[QF32 ? blk : 0], c);
@@ -313,26 +337,64 @@ __global__ void __launch_bounds__(64 * kWaves) part_kernel(PartArgs a) {
                     *reinterpret_cast<float4*>(to + 16 * J) = make_float4(s[J][0], s[J][1], s[J][2], s[J][3]);
             }
         }
+        if (next) load_k(row);
+        // V's scales: those of keys that no column sees may hold anything, non-finite values
+        // too; the largest of the others bounds `shift`.
+        if constexpr (!VF16) {
+            ScaleVec x = vsc;
+            if (!whole) {
+                const uint32_t t = tok0 + lane / 2;
+                if (t >= L || (t < vis.lo && t >= a.sinks)) x = ScaleVec{};
+            }
+            asm volatile("" ::: "memory");
+            *reinterpret_cast<ScaleVec*>(s_sc + kChunk * NB + lane * (NB / 2)) = x;
+            asm volatile("" ::: "memory");
+            // positive fp16 numbers are ordered as their bits (a sign counts as large)
+            const uint32_t* xw = reinterpret_cast<const uint32_t*>(&x);
+            uint32_t bits = 0;
+#pragma unroll
+            for (uint32_t w = 0; w < NB / 4; ++w) bits = max(bits, max(xw[w] & 0xffffu, xw[w] >> 16));
+            // a scale of exponent field f is below 2^(f - 14)
+            if (__any(static_cast<int>(bits >> 10) - 14 + shift > 15)) {
+                uint32_t top = bits;
+#pragma unroll
+                for (uint32_t off = 1; off < 64; off <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, 64)));
+                const int fits = max(kMinShift, 15 + 14 - static_cast<int>(__builtin_amdgcn_readfirstlane(top) >> 10));
+                if (fits < shift) {
+                    const float f = exp2_fast(static_cast<float>(fits - shift));
+                    ref += static_cast<float>(shift - fits);
+                    shift = fits;
+                    if (!fresh) {
+                        l_run *= f;
+#pragma unroll
+                        for (uint32_t mt = 0; mt < NM; ++mt) O[mt] *= f;
+                    }
+                }
+            }
+        }
         // Online softmax: the running maximum, rescaled where it grows.
         float top = s[0][0];
 #pragma unroll
         for (uint32_t J = 0; J < 2; ++J)
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k) top = fmaxf(top, s[J][k]);
-        top = rows_reduce(top, MaxOp{});
-        if (__any(top > m_run)) {
-            const float m_new = fmaxf(m_run, top);
-            const float f = m_run == -INFINITY ? 0.0f : exp2_fast(m_run - m_new);
-            m_run = m_new;
-            l_run *= f;
+        top = rows_reduce(top, MaxOp{}) - static_cast<float>(shift);
+        if (__any(top > ref)) {
+            const float to_ref = fmaxf(ref, top);
+            if (!fresh) {
+                const float f = ref == -INFINITY ? 0.0f : exp2_fast(ref - to_ref);
+                l_run *= f;
 #pragma unroll
-            for (uint32_t mt = 0; mt < NM; ++mt) O[mt] *= f;
+                for (uint32_t mt = 0; mt < NM; ++mt) O[mt] *= f;
+            }
+            ref = to_ref;
         }
-        const float m_use = m_run == -INFINITY ? 0.0f : m_run;  // a column that saw no key yet
+        fresh = false;
+        const float use = ref == -INFINITY ? 0.0f : ref;  // a column that saw no key yet
         float p[8];
 #pragma unroll
         for (uint32_t x = 0; x < 8; ++x) {
-            p[x] = exp2_fast(s[x / 4][x % 4] - m_use + kPShift);
+            p[x] = exp2_fast(s[x / 4][x % 4] - use);
             l_run += p[x];
         }
         // O^T += V^T P^T; element 8 g4 + x of the MFMA's K axis is key 16 (x / 4) + 4 g4 + x % 4,
@@ -346,7 +408,7 @@ __global__ void __launch_bounds__(64 * kWaves) part_kernel(PartArgs a) {
             }
 #pragma unroll
             for (uint32_t mt = 0; mt < NM; ++mt) {
-                half8 v = __builtin_bit_cast(half8, st.v[mt]);
+                half8 v = __builtin_bit_cast(half8, vreg[mt]);
                 if (!whole) {
 #pragma unroll
                     for (uint32_t x = 0; x < 8; ++x) {
@@ -370,29 +432,24 @@ __global__ void __launch_bounds__(64 * kWaves) part_kernel(PartArgs a) {
                 half8 hi, lo;
 #pragma unroll
                 for (uint32_t x = 0; x < 8; ++x) {
-                    const float ps = p[x] * f16_bits_to_f32(sc[(x / 4) * 4 * NB + (x % 4) * NB + blk]);
+                    float ps = p[x] * f16_bits_to_f32(sc[(x / 4) * 4 * NB + (x % 4) * NB + blk]);
+                    // both parts come from the rounded product: hi taken from the exact one (a
+                    // fused multiply and conversion) now and then rounds the other way, and lo
+                    // does not make up for it (outputs 5e-6 off)
+                    asm("" : "+v"(ps));
                     hi[x] = static_cast<_Float16>(ps);
                     lo[x] = static_cast<_Float16>(ps - static_cast<float>(hi[x]));
                 }
 #pragma unroll
                 for (uint32_t mt = 2 * blk; mt < 2 * blk + 2; ++mt) {
-                    const uint2 vw = __builtin_bit_cast(uint2, st.v[mt]);
+                    const uint2 vw = __builtin_bit_cast(uint2, vreg[mt]);
                     const half8 v = codes8_to_half8(vw.x, vw.y);
                     O[mt] = mfma_16x16x32(v, hi, O[mt]);
                     O[mt] = mfma_16x16x32(v, lo, O[mt]);
                 }
             }
         }
-    };
-
-    {
-        Step st;
-        for (uint32_t j = 0; j < run.cpw; ++j) {
-            const uint32_t i = first + wave + kWaves * j;
-            if (i >= total) break;  // wave-uniform
-            load_step(i, st);
-            compute(i, st);
-        }
+        if (next) load_v(row);
     }
     l_run = rows_reduce(l_run, AddOp{});
 
@@ -403,7 +460,7 @@ __global__ void __launch_bounds__(64 * kWaves) part_kernel(PartArgs a) {
     float* s_o = smem + kWaves * 32;   // [kWaves][cols][D]
     if (col) {
         if (g4 == 0) {
-            s_m[wave * 16 + n] = m_run;
+            s_m[wave * 16 + n] = ref;
             s_l[wave * 16 + n] = l_run;
         }
 #pragma unroll
@@ -458,7 +515,7 @@ __device__ void merge_records(const PartArgs& a) {
     float4 gv = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (a.gate != nullptr) gv = *reinterpret_cast<const float4*>(a.gate + at);
     uint32_t first, runs;
-    find_records(a, b, h, first, runs);
+    find_records(a, bh, b, first, runs);
     const uint32_t rec = part_record(a.cols, D);
     const float* base = a.part + static_cast<size_t>(first) * rec;
     float m = -INFINITY, l = 0.0f;
@@ -512,7 +569,7 @@ template <uint32_t D>
 __device__ void add_weights(const PartArgs& a, uint32_t x) {
     const uint32_t blocks = (a.max_context + kWeightKeys - 1) / kWeightKeys;
     const uint32_t bh = x / blocks, key = (x % blocks) * kWeightKeys + threadIdx.x;
-    const uint32_t b = bh / a.g.kv_heads, h = bh % a.g.kv_heads;
+    const uint32_t b = bh / a.g.kv_heads;
     const uint32_t L = part_length(a, b);
     if ((x % blocks) * kWeightKeys >= L) return;  // workgroup-uniform
     // the scores go out ahead of the records
@@ -526,7 +583,7 @@ __device__ void add_weights(const PartArgs& a, uint32_t x) {
     __shared__ float s_m[16][16], s_l[16][16];
     const uint32_t c = threadIdx.x & 15, rg = threadIdx.x >> 4;
     uint32_t first, runs;
-    find_records(a, b, h, first, runs);
+    find_records(a, bh, b, first, runs);
     const uint32_t rec = part_record(a.cols, D);
     float m = -INFINITY, l = 0.0f;
     if (c < a.cols)
@@ -548,8 +605,7 @@ __device__ void add_weights(const PartArgs& a, uint32_t x) {
             m = mn;
         }
         s_m[0][c] = m == -INFINITY ? 0.0f : m;
-        // l carries P's scale
-        s_l[0][c] = l > 0.0f ? exp2f(kPShift) / l : 0.0f;
+        s_l[0][c] = l > 0.0f ? 1.0f / l : 0.0f;
     }
     __syncthreads();
     float sum = 0.0f;
@@ -571,6 +627,7 @@ __global__ void __launch_bounds__(256) part_finish_kernel(PartArgs a) {
 }
 
 struct PartPlan {
+    uint64_t run_bytes;
     uint64_t wgs;        // of the first launch: an upper bound on the runs
     uint64_t part_bytes;
     uint64_t logit_bytes;
@@ -587,6 +644,7 @@ PartPlan part_plan(const miikv_view* v, uint32_t q_heads, uint32_t batch, uint32
     // the runs: at most the target and one partial run per pair, or one step per wave
     p.wgs = std::min<uint64_t>(kTargetWgs + pairs, pairs * ((most + kWaves - 1) / kWaves));
     const uint32_t cols = q_heads / v->kv_heads * tokens;
+    p.run_bytes = up256(pairs * 2 * sizeof(uint32_t));
     p.part_bytes = up256(p.wgs * part_record(cols, v->head_dim) * sizeof(float));
     p.logit_keys = (max_context + kChunk - 1) / kChunk * kChunk;
     p.logit_bytes = scored ? up256(pairs * cols * p.logit_keys * sizeof(float)) : 0u;
@@ -636,7 +694,7 @@ miikv_status part_impl(const miikv_view* view, const void* q, uint32_t q_dtype, 
     if (window >= max_context) window = 0;  // hides nothing
     sinks = std::min(sinks, max_context);
     const PartPlan p = part_plan(view, q_heads, batch, tokens, max_context, window, sinks, scored);
-    if (workspace == nullptr || workspace_bytes < p.part_bytes + p.logit_bytes) return MIIKV_EWORKSPACE;
+    if (workspace == nullptr || workspace_bytes < p.run_bytes + p.part_bytes + p.logit_bytes) return MIIKV_EWORKSPACE;
 
     PartArgs a{};
     a.g = make_geo(*view);
@@ -654,8 +712,10 @@ miikv_status part_impl(const miikv_view* view, const void* q, uint32_t q_dtype, 
     a.sinks = sinks;
     a.batch = batch;
     a.target_wgs = kTargetWgs;
-    a.part = static_cast<float*>(workspace);
-    a.logits = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.part_bytes);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    a.runs = reinterpret_cast<uint32_t*>(ws);
+    a.part = reinterpret_cast<float*>(ws + p.run_bytes);
+    a.logits = reinterpret_cast<float*>(ws + p.run_bytes + p.part_bytes);
     a.logit_keys = p.logit_keys;
     a.weights = weights;
     a.weight_stride = weight_stride;
@@ -692,7 +752,8 @@ extern "C" uint64_t miikv_window_workspace_bytes(const miikv_view* view, uint32_
                                                  uint32_t max_context, uint32_t window, uint32_t sinks) {
     if (part_sizes(view, q_heads, batch, tokens, max_context) != MIIKV_OK) return 0;
     if (window >= max_context) window = 0;
-    return part_plan(view, q_heads, batch, tokens, max_context, window, std::min(sinks, max_context), false).part_bytes;
+    const PartPlan p = part_plan(view, q_heads, batch, tokens, max_context, window, std::min(sinks, max_context), false);
+    return p.run_bytes + p.part_bytes;
 }
 
 extern "C" miikv_status miikv_decode_attn_window(const miikv_view* view, const void* q, uint32_t q_dtype, uint32_t q_heads,
@@ -709,7 +770,7 @@ extern "C" uint64_t miikv_scored_workspace_bytes(const miikv_view* view, uint32_
                                                  uint32_t max_context) {
     if (part_sizes(view, q_heads, batch, tokens, max_context) != MIIKV_OK) return 0;
     const PartPlan p = part_plan(view, q_heads, batch, tokens, max_context, 0, 0, true);
-    return p.part_bytes + p.logit_bytes;
+    return p.run_bytes + p.part_bytes + p.logit_bytes;
 }
 
 extern "C" miikv_status miikv_decode_attn_scored(const miikv_view* view, const void* q, uint32_t q_dtype, uint32_t q_heads,
