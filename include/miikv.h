@@ -72,7 +72,7 @@ enum { MIIKV_LAYOUT_CONTIGUOUS = 0, MIIKV_LAYOUT_PAGED = 1 };
  * MIIKV_EUNSUPPORTED otherwise). */
 enum { MIIKV_KV_FP16_FP16 = 0, MIIKV_KV_Q8_FP16 = 1, MIIKV_KV_FP16_Q8 = 2, MIIKV_KV_Q8_Q8 = 3 };
 
-enum { MIIKV_DTYPE_F16 = 0, MIIKV_DTYPE_F32 = 1 };
+enum { MIIKV_DTYPE_F16 = 0, MIIKV_DTYPE_F32 = 1, MIIKV_DTYPE_BF16 = 2 /* miikv_chunk_attn only */ };
 
 /* Non-owning view of one attention layer's KV cache.
  * Replaces AttentionKvCacheView (include/miinfer/prefill_v2/kv_cache.hpp:24-46),
@@ -374,6 +374,32 @@ miikv_status miikv_suffix_attn_ex(const miikv_view* view, const uint16_t* k_new,
  * a context shorter than its tokens) gets zeros.  Pages whose keys no token of the
  * call sees are not read: their table entries may be -1.  No counterpart in the
  * reference, whose attention layers see the whole context. */
+
+/* Attention of a ragged batch of chunks of new tokens (prompts' chunks, chat turns,
+ * drafted tokens and single decode steps mixed in one call) over a paged cache, or of
+ * one chunk over a contiguous one, causal, with the window above.  The new tokens' rows
+ * are in the cache.
+ *   q / out  device [total_tokens][q_heads][head_dim], the sequences' chunks one behind
+ *        the other: sequence b's are rows d_offsets[b] .. d_offsets[b + 1] - 1.  q_dtype and
+ *        out_dtype are MIIKV_DTYPE_F16, _BF16 or _F32, not necessarily the same.  Rows of
+ *        out that belong to no chunk stay as they were.
+ *   d_offsets device [batch + 1], ascending; d_lengths device [batch]: context lengths, the
+ *        new tokens included.  A chunk may be empty.
+ *   max_tokens, max_context  host upper bounds of a chunk and a context; what exceeds them
+ *        (or total_tokens) is left out.
+ * Precision: query, dequantised keys and values, and probabilities are rounded to fp16
+ * once, sums and statistics are fp32 (about 4e-4 of the outputs' norm; an fp32 out shows
+ * it).  A value that is not finite spreads to the call's tokens that see another key of
+ * its 32-key step.  miikv_chunk_workspace_bytes() is 0 for arguments that the call
+ * refuses; MIIKV_EUNSUPPORTED for batches whose plan does not fit a workgroup's LDS
+ * (about 16000 items of 256 (token, query head) rows). */
+uint64_t miikv_chunk_workspace_bytes(const miikv_view* view, uint32_t q_heads, uint32_t batch, uint32_t total_tokens,
+                                     uint32_t max_tokens, uint32_t max_context, uint32_t window, uint32_t sinks);
+miikv_status miikv_chunk_attn(const miikv_view* view, const void* q, uint32_t q_dtype, uint32_t q_heads, float scale,
+                              uint32_t batch, uint32_t total_tokens, const uint32_t* d_offsets,
+                              const uint32_t* d_lengths, uint32_t max_tokens, uint32_t max_context, uint32_t window,
+                              uint32_t sinks, void* out, uint32_t out_dtype, void* workspace, uint64_t workspace_bytes,
+                              void* stream);
 
 /* Decode attention with a sliding window: the last `tokens` tokens of each sequence
  * (1: a decode step; more: drafted tokens being verified), whose rows the cache holds.

@@ -6,6 +6,8 @@ gfx950) and fails loudly when that library is missing.
 """
 from ._lib import MiikvError, lib  # noqa: F401
 from .bounded import (  # noqa: F401
+    chunk_attention,
+    chunk_workspace_bytes,
     evict,
     scored_attention,
     scored_workspace_bytes,
@@ -28,5 +30,6 @@ from .kv import (  # noqa: F401
 __all__ = [
     "MiikvError", "lib", "advance_decode_state", "KvCache", "DecodeWorkspace", "decode_attention", "clone_state",
     "copy_segments", "make_decode_state", "make_prefill_state", "suffix_attention", "suffix_workspace_bytes",
-    "evict", "scored_attention", "scored_workspace_bytes", "window_attention", "window_workspace_bytes",
+    "chunk_attention", "chunk_workspace_bytes", "evict", "scored_attention", "scored_workspace_bytes", "window_attention",
+    "window_workspace_bytes",
 ]

@@ -30,6 +30,7 @@ SUFFIX_EXACT = 2  # MIIKV_SUFFIX_EXACT
 
 DTYPE_F16 = 0
 DTYPE_F32 = 1
+DTYPE_BF16 = 2  # miikv_chunk_attn only
 
 
 class MiikvView(ctypes.Structure):
@@ -117,6 +118,9 @@ SIGNATURES = {
     "miikv_pool_prepare_append": (ctypes.c_int, [_P, _P, _U32, _U32, _U32, _P, _P, _P]),
     "miikv_pool_release": (ctypes.c_int, [_P, _P, _U32, _U32]),
     "miikv_pool_truncate": (ctypes.c_int, [_P, _P, _U32, _U32, _U32]),
+    "miikv_chunk_workspace_bytes": (_U64, [_VP, _U32, _U32, _U32, _U32, _U32, _U32, _U32]),
+    "miikv_chunk_attn": (ctypes.c_int, [_VP, _P, _U32, _U32, ctypes.c_float, _U32, _U32, _P, _P, _U32, _U32, _U32, _U32,
+                                         _P, _U32, _P, _U64, _P]),
     "miikv_window_workspace_bytes": (_U64, [_VP, _U32, _U32, _U32, _U32, _U32, _U32]),
     "miikv_decode_attn_window": (ctypes.c_int, [_VP, _P, _U32, _U32, ctypes.c_float, _U32, _U32, _P, _P, _U32, _U32,
                                                  _U32, _P, _P, _P, _P, _U64, _P]),

@@ -1,7 +1,8 @@
 """Attention over part of a cache, and caches that are made smaller.
 
-``window_attention`` is decode attention with a sliding window and the first tokens that
-stay visible, ``scored_attention`` decode attention that adds up the weight every key
+``chunk_attention`` is attention of a ragged batch of chunks of new tokens, over the whole
+cache or a sliding window and the first tokens that stay visible, ``window_attention`` its
+form for single tokens, ``scored_attention`` decode attention that adds up the weight every key
 gets, ``evict`` keeps the keys with the largest weights and moves their rows together.
 Every call goes through libmiikv; there is no fallback path.  The reference has no
 counterpart: its attention layers keep and see the whole context.
@@ -87,6 +88,61 @@ def _workspace(need: int, q: torch.Tensor) -> torch.Tensor:
     if need == 0:
         raise ValueError("the sizes are not ones that this call serves")
     return torch.empty(need, dtype=torch.uint8, device=q.device)
+
+
+_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
+
+
+def chunk_workspace_bytes(cache: KvCache, q_heads: int, batch: int, total_tokens: int, max_tokens: int, max_context: int,
+                          window: int = 0, sinks: int = 0) -> int:
+    return int(lib().miikv_chunk_workspace_bytes(cache.view, q_heads, batch, total_tokens, max_tokens, max_context, window, sinks))
+
+
+def chunk_attention(cache: KvCache, q: torch.Tensor, offsets: torch.Tensor, lengths: torch.Tensor,
+                    scale: float | None = None, *, max_tokens: int | None = None, max_context: int | None = None,
+                    window: int = 0, sinks: int = 0, out: torch.Tensor | None = None,
+                    workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Causal attention of a ragged batch of chunks of new tokens, whose rows the cache holds:
+    prompts' chunks, chat turns, drafted tokens and single steps in one call.
+
+    q: [total_tokens, q_heads, head_dim], fp16, bf16 or fp32; sequence b's tokens are rows
+    offsets[b] .. offsets[b + 1] - 1 (device int32 [batch + 1]) and end its context of
+    lengths[b] keys (device int32 [batch]).  With `window` the token at position p sees the
+    keys j <= p with j > p - window or j < sinks.  max_tokens and max_context bound a chunk and
+    a context (by default total_tokens and the cache's capacity; nearer bounds make smaller
+    workspaces).  Returns `out` ([total_tokens, q_heads, head_dim], fp16, bf16 or fp32; by
+    default of q's type); rows that belong to no chunk stay as they were."""
+    if q.dim() != 3 or q.shape[-1] != cache.head_dim or q.dtype not in _DTYPES:
+        raise ValueError("q must be fp16/bf16/fp32 [total_tokens, q_heads, head_dim]")
+    total, q_heads = q.shape[0], q.shape[1]
+    batch = lengths.numel()
+    if lengths.dtype not in _INDEX or offsets.dtype not in _INDEX or offsets.numel() != batch + 1:
+        raise ValueError("offsets and lengths must be int32 [batch + 1] and [batch]")
+    if out is not None and (out.shape != q.shape or out.dtype not in _DTYPES):
+        raise ValueError("out must be fp16/bf16/fp32, of q's shape")
+    _check(cache, stream, q=q, offsets=offsets, lengths=lengths, out=out, workspace=workspace)
+    _check_batch(cache, batch)
+    if max_context is None:
+        max_context = cache.capacity
+    if max_tokens is None:
+        max_tokens = min(total, max_context)
+    _u32_arg("max_tokens", max_tokens, 1)
+    _u32_arg("max_context", max_context, 1)
+    _u32_arg("window", window)
+    _u32_arg("sinks", sinks)
+    with _on_device(cache.k_codes.device):
+        if workspace is None or out is None:
+            with _on_stream(stream):
+                if workspace is None:
+                    workspace = _workspace(chunk_workspace_bytes(cache, q_heads, batch, total, max_tokens, max_context, window,
+                                                                 sinks), q)
+                if out is None:
+                    out = torch.empty_like(q)
+        call("miikv_chunk_attn", cache.view, q.data_ptr(), _DTYPES[q.dtype], q_heads,
+             1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale), batch, total, offsets.data_ptr(),
+             lengths.data_ptr(), max_tokens, max_context, window, sinks, out.data_ptr(), _DTYPES[out.dtype],
+             workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(stream))
+    return out
 
 
 def window_workspace_bytes(cache: KvCache, q_heads: int, batch: int, tokens: int, max_context: int, window: int,

@@ -21,6 +21,7 @@ SOURCES = [
     "miikv_decode.hip",
     "miikv_suffix.hip",
     "miikv_window.hip",
+    "miikv_chunk.hip",
     "miikv_evict.hip",
     "miikv_host.cpp",
     "miikv_session.cpp",

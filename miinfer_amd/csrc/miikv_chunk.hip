@@ -1,0 +1,722 @@
+// Attention of a ragged batch of chunks of new tokens over a paged cache, causal, with an
+// optional sliding window and the first tokens (gfx950, wave64, MFMA).
+//
+// Token t of sequence b's n_b new ones stands at p = L_b - n_b + t and sees the keys j <= p
+// with j > p - window (window == 0: all) or j < sinks:
+//   s_j = scale * q . k_j,  o = sum_j e^{s_j - m} v_j / sum_j e^{s_j - m}.
+//
+// Work.  The rows of a (sequence, kv head) are its (token, query head of the group) pairs;
+// kRows of them are an item, whose tokens together see a run of 32-key steps (and the steps
+// of the first tokens).  Items differ in length (short chunks, causality, windows), so the
+// items of all kv heads are laid on one axis, kItemCost units and one per step each, and the
+// axis is cut into equal parts, one per workgroup of the one resident round: every CU has the
+// same work whatever the lengths are.  An item that lies in one part is written straight
+// to the output; the parts of one that is cut leave records, which the second launch merges.
+//
+// A workgroup's eight waves own 32 rows each and share the key tiles in LDS.  Per step
+//   S^T[key][row] = K (32 keys x D) Q^T,  O^T[dim][row] += V^T (dims x 32 keys) P^T
+// with v_mfma_f32_32x32x16_f16: S's result layout (a lane holds 16 keys of one row) is the B
+// operand of the second product as it stands.  Steps come into a ring in LDS as the cache holds
+// them, by copies that pass no registers (at D = 256 O^T and the query take 192 of the 256);
+// the next step's codes are turned into fp16 rows (code * scale, rounded once) in the other tile
+// buffer before this step's tile is multiplied.
+//
+// Precision: query, code * scale and probabilities are fp16, sums and statistics fp32,
+// the records' normalised outputs fp16.
+#include "miikv_part.hpp"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace miikv {
+namespace {
+
+constexpr uint32_t kChunkWaves = 8;
+constexpr uint32_t kChunkThreads = 64 * kChunkWaves;
+constexpr uint32_t kRows = 32 * kChunkWaves;  // rows of an item
+constexpr uint32_t kItemCost = 4;             // an item's fixed cost, in steps
+constexpr uint32_t kMinUnits = 12;            // units per workgroup, at least
+constexpr uint32_t kMaxParts = 256;           // one workgroup per CU
+constexpr float kSlack = 8.0f;                // the maximum may grow by this (log2) before sums are rescaled
+
+struct ChunkItem {
+    uint32_t b;      // sequence
+    uint32_t rows0;  // its first row
+    uint32_t start;  // units of one kv head before it
+    uint32_t steps;
+};
+
+struct ChunkArgs {
+    Geo g;
+    const void* q;
+    uint32_t q_dtype;
+    uint32_t q_heads;
+    uint32_t group;  // query heads per kv head
+    float scale_log2;  // above 0: a negative scale negates the query
+    uint32_t negate;
+    uint32_t batch;
+    uint32_t total_tokens;
+    uint32_t max_tokens;
+    uint32_t max_context;
+    uint32_t window;
+    uint32_t sinks;
+    const uint32_t* offsets;
+    const uint32_t* lengths;
+    void* out;
+    uint32_t out_dtype;
+    uint32_t most_items;  // of one kv head
+    uint32_t parts;
+    // workspace
+    uint32_t* head;      // [0] items of one kv head, [1] units of one kv head, [2] units per part
+    ChunkItem* items;    // [most_items]
+    _Float16* rec_o;     // [2 * parts][kRows][D]: outputs over the part's keys
+    float2* rec_ml;      // [2 * parts][kRows]: maximum (log2 units) and sum
+};
+
+// Sequence b's chunk: its first row in q, its tokens and its context, all within the bounds
+// that the host knows (so that wrong device data reads and writes no further).
+struct Chunk {
+    uint32_t q0, tokens, length;
+};
+__device__ __forceinline__ Chunk chunk_of(const ChunkArgs& a, uint32_t b) {
+    Chunk c;
+    c.q0 = min(a.offsets[b], a.total_tokens);
+    const uint32_t end = min(a.offsets[b + 1], a.total_tokens);
+    c.tokens = end > c.q0 ? min(end - c.q0, a.max_tokens) : 0u;
+    c.length = min(a.lengths[b], a.max_context);
+    return c;
+}
+
+// chunk_of a wave-uniform b, in scalar registers.
+__device__ __forceinline__ Chunk chunk_of_uniform(const ChunkArgs& a, uint32_t b) {
+    Chunk c;
+    c.q0 = min(scalar_load(a.offsets + b), a.total_tokens);
+    const uint32_t end = min(scalar_load(a.offsets + b + 1), a.total_tokens);
+    c.tokens = end > c.q0 ? min(end - c.q0, a.max_tokens) : 0u;
+    c.length = min(scalar_load(a.lengths + b), a.max_context);
+    return c;
+}
+// Workgroup barrier after this wave's LDS reads have returned and its writes are done;
+// copies to LDS stay in flight.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// What the rows rows0 .. of a chunk see together: the context of the last of them, their
+// tokens and the steps.
+struct Span {
+    uint32_t rows;   // of the item
+    uint32_t past;   // keys up to the last token's own
+    uint32_t tokens;
+    Visible vis;
+};
+__device__ __forceinline__ Span span_of(const ChunkArgs& a, const Chunk& c, uint32_t rows0) {
+    Span s;
+    s.rows = min(kRows, c.tokens * a.group - rows0);
+    const uint32_t t0 = rows0 / a.group, t1 = (rows0 + s.rows - 1) / a.group;
+    s.past = c.length + t1 + 1 > c.tokens ? c.length + t1 + 1 - c.tokens : 0u;
+    s.tokens = t1 - t0 + 1;
+    s.vis = visible_steps(s.past, s.tokens, a.window, a.sinks);
+    return s;
+}
+
+// Inclusive sums over the workgroup's threads; `total` is the last one's.
+__device__ __forceinline__ uint32_t scan_threads(uint32_t x, uint32_t* s_wave, uint32_t& total) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t incl = x;
+#pragma unroll
+    for (uint32_t off = 1; off < 64; off <<= 1) {
+        const uint32_t up = __shfl_up(incl, off, 64);
+        if (lane >= off) incl += up;
+    }
+    __syncthreads();
+    if (lane == 63) s_wave[wave] = incl;
+    __syncthreads();
+    total = 0;
+    uint32_t before = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kChunkWaves; ++w) {
+        if (w < wave) before += s_wave[w];
+        total += s_wave[w];
+    }
+    return before + incl;
+}
+
+__device__ __forceinline__ float16v mfma_32x32x16(half8 a, half8 b, float16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+// `use`(c, t[c * stride]) for c < N; the next pair of fragments is on its way from LDS while
+// a pair's MFMAs run.
+template <uint32_t N, typename F>
+__device__ __forceinline__ void mfma_pairs(const half8* t, uint32_t stride, F use) {
+    half8 f[2][2] = {{t[0], t[stride]}, {}};
+#pragma unroll
+    for (uint32_t c = 0; c < N; c += 2) {
+        const uint32_t k = (c / 2) & 1;
+        if (c + 2 < N) {
+            f[k ^ 1][0] = t[(c + 2) * stride];
+            f[k ^ 1][1] = t[(c + 3) * stride];
+        }
+        __builtin_amdgcn_sched_barrier(0);  // the scheduler would move the reads to their use, or all of them up here
+        use(c, f[k][0]);
+        use(c + 1, f[k][1]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// `use`(zero of the type that `dtype` names): one branch per loop, not per element.
+template <typename F>
+__device__ __forceinline__ void with_type(uint32_t dtype, F use) {
+    if (dtype == MIIKV_DTYPE_BF16) use(__bf16{});
+    else if (dtype == MIIKV_DTYPE_F16) use(_Float16{});
+    else use(float{});
+}
+// Four values to element `at` of an array of T, rounded to nearest even.
+template <typename T>
+__device__ __forceinline__ void store4(void* out, size_t at, float4 x) {
+    typedef T vec __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<vec*>(static_cast<T*>(out) + at) =
+        vec{static_cast<T>(x.x), static_cast<T>(x.y), static_cast<T>(x.z), static_cast<T>(x.w)};
+}
+// Eight query values, rounded to fp16.
+template <typename T>
+__device__ __forceinline__ half8 load_query(const void* q, size_t at) {
+    typedef T vec __attribute__((ext_vector_type(8)));
+    const vec x = *reinterpret_cast<const vec*>(static_cast<const T*>(q) + at);
+    if constexpr (std::is_same<T, _Float16>::value) {
+        return x;
+    } else {
+        half8 r;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = static_cast<_Float16>(static_cast<float>(x[i]));
+        return r;
+    }
+}
+
+// A block scale of a tile: 128 * 511.75 = 65504 is the largest that leaves every code finite.
+// (Larger ones stand for blocks within 0.8% of fp16's maximum.)
+__device__ __forceinline__ _Float16 tile_scale(uint16_t bits) {
+    return __builtin_elementwise_min(__builtin_bit_cast(_Float16, bits), static_cast<_Float16>(511.75f));
+}
+
+// LDS of chunk_kernel: two fp16 tiles of a step, K units [D / 8][32 keys] and V units [4][D + 4]
+// of 8 values (V's rows of units are 64 bytes longer than they need be: neighbouring threads
+// write units of two rows), and a ring of steps as the cache holds them: K codes, V codes, K
+// scales, V scales.
+template <uint32_t D, bool KF16, bool VF16>
+struct ChunkLds {
+    static constexpr uint32_t k_units = D / 8 * kChunk;
+    static constexpr uint32_t v_row = D + 4;
+    static constexpr uint32_t units = k_units + 4 * v_row;
+    static constexpr uint32_t k_bytes = kChunk * D * (KF16 ? 2 : 1), v_bytes = kChunk * D * (VF16 ? 2 : 1);
+    static constexpr uint32_t scale_bytes = kChunk * (D / 32) * 2;
+    static constexpr uint32_t raw = k_bytes + v_bytes + 2 * scale_bytes;
+    // Steps of the ring, as far as 160 KB go; how many steps ahead of the one being multiplied
+    // must have landed (V's scales are put in order a step before its codes are converted); and
+    // the copies that each wave issues per step (with scales of one plane only, four waves issue
+    // one less, so those modes wait for all copies).
+    static constexpr uint32_t bufs = D == 128 || !(KF16 || VF16) ? 4 : (KF16 && VF16 ? 2 : 3);
+    static constexpr uint32_t landed = VF16 ? 1 : 2;
+    static constexpr uint32_t ops = (k_bytes + v_bytes) / 1024 / kChunkWaves + (KF16 && VF16 ? 0 : 1);
+    static constexpr uint32_t vsc_bytes = 2 * 2 * D;  // V's scales of two steps in the order of its units
+    static constexpr uint32_t bytes = 2 * units * 16 + bufs * raw + vsc_bytes;
+};
+
+template <uint32_t D, bool KF16, bool VF16>
+__global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(2))) chunk_kernel(ChunkArgs a) {
+    constexpr uint32_t NB = D / 32;
+    constexpr uint32_t NQ = D / 16;  // K-axis chunks of the first product
+    constexpr uint32_t KE = KF16 ? 2 : 1, VE = VF16 ? 2 : 1;
+    using Lds = ChunkLds<D, KF16, VF16>;
+    extern __shared__ __align__(16) uint8_t lds[];
+    half8* const s_tile = reinterpret_cast<half8*>(lds);  // two tiles
+    uint8_t* const s_raw = lds + 2 * Lds::units * 16;
+    _Float16* const s_vsc = reinterpret_cast<_Float16*>(s_raw + Lds::bufs * Lds::raw);  // [2][NB][4][8]
+    uint32_t* const s_first = reinterpret_cast<uint32_t*>(lds + Lds::bytes);  // [batch + 1]: items before sequence b
+    uint32_t* const s_start = s_first + a.batch + 1;                          // [most_items + 1]: units before item i
+    __shared__ uint32_t s_wave[kChunkWaves];
+
+    const uint32_t tid = threadIdx.x, lane = tid & 63, n = lane & 31, hh = lane >> 5;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Geo& geo = a.g;
+
+    // ---- the plan, by every workgroup for itself
+    uint32_t base = 0, total;
+    for (uint32_t b0 = 0; b0 < a.batch; b0 += kChunkThreads) {
+        const uint32_t b = b0 + tid;
+        const uint32_t mine = b < a.batch ? (chunk_of(a, b).tokens * a.group + kRows - 1) / kRows : 0u;
+        const uint32_t incl = scan_threads(mine, s_wave, total);
+        if (b < a.batch) s_first[b] = base + incl - mine;
+        base += total;
+    }
+    const uint32_t items = uniform(min(base, a.most_items));
+    if (tid == 0) s_first[a.batch] = base;
+    __syncthreads();
+    uint32_t units = 0;
+    for (uint32_t i0 = 0; i0 < items; i0 += kChunkThreads) {
+        const uint32_t i = i0 + tid;
+        uint32_t mine = 0;
+        ChunkItem it{};
+        if (i < items) {
+            uint32_t lo = 0, hi = a.batch;  // the last sequence whose items start at or before i
+            while (hi - lo > 1) {
+                const uint32_t mid = (lo + hi) / 2;
+                if (s_first[mid] <= i) lo = mid;
+                else hi = mid;
+            }
+            it.b = lo;
+            it.rows0 = (i - s_first[lo]) * kRows;
+            it.steps = span_of(a, chunk_of(a, lo), it.rows0).vis.steps();
+            mine = kItemCost + it.steps;
+        }
+        const uint32_t incl = scan_threads(mine, s_wave, total);
+        if (i < items) {
+            it.start = units + incl - mine;
+            s_start[i] = it.start;
+            if (blockIdx.x == 0) a.items[i] = it;
+        }
+        units += total;
+    }
+    units = uniform(units);
+    const uint32_t axis = units * geo.kv_heads;  // the host has seen that it fits 32 bits
+    const uint32_t quota = uniform(max(axis / a.parts + (axis % a.parts != 0 ? 1u : 0u), kMinUnits));
+    if (tid == 0) {
+        s_start[items] = units;
+        if (blockIdx.x == 0) {
+            a.head[0] = items;
+            a.head[1] = units;
+            a.head[2] = quota;
+        }
+    }
+    __syncthreads();
+    // Parts that follow each other on the axis read the same keys: they go to one XCD (workgroup
+    // w runs on XCD w % 8).
+    const uint32_t per = (a.parts + 7) / 8;
+    const uint32_t part = (blockIdx.x % 8) * per + blockIdx.x / 8;
+    if (part >= a.parts) return;
+    if (static_cast<uint64_t>(part) * quota >= axis) return;
+    const uint32_t begin = part * quota, end = axis - begin < quota ? axis : begin + quota;
+    uint32_t at = begin;
+
+    while (at < end) {
+        const uint32_t h = uniform(at / units);
+        const uint32_t in_head = at - h * units;
+        uint32_t i = 0;
+        {
+            uint32_t hi = items;
+            while (hi - i > 1) {
+                const uint32_t mid = (i + hi) / 2;
+                if (uniform(s_start[mid]) <= in_head) i = mid;
+                else hi = mid;
+            }
+        }
+        uint32_t b = 0;
+        {
+            uint32_t hi = a.batch;
+            while (hi - b > 1) {
+                const uint32_t mid = (b + hi) / 2;
+                if (uniform(s_first[mid]) <= i) b = mid;
+                else hi = mid;
+            }
+        }
+        const uint32_t start = h * units + uniform(s_start[i]), stop = h * units + uniform(s_start[i + 1]);
+        const Chunk c = chunk_of_uniform(a, b);
+        const uint32_t rows0 = (i - uniform(s_first[b])) * kRows;
+        Span span = span_of(a, c, rows0);
+        // (the divisions by the group leave these in vector registers)
+        span.rows = uniform(span.rows);
+        span.past = uniform(span.past);
+        span.vis = {uniform(span.vis.head), uniform(span.vis.first), uniform(span.vis.end), uniform(span.vis.lo)};
+        const uint32_t steps = span.vis.steps();
+        const uint32_t first = start + kItemCost;  // the axis place of its first step
+        const uint32_t s0 = uniform(at > first ? at - first : 0u);
+        const uint32_t s1 = uniform(end > first ? min(end - first, steps) : 0u);
+        at = stop;
+        if (s0 >= s1 && !(steps == 0 && start >= begin)) continue;  // only some of its fixed cost is here
+
+        // ---- this wave's rows
+        const uint32_t r = wave * 32 + n;  // of the item
+        const bool row_live = r < span.rows;
+        const uint32_t row = rows0 + min(r, span.rows - 1);
+        const uint32_t tok = row / a.group, head = h * a.group + (row - tok * a.group);
+        const uint32_t past = c.length + tok + 1 > c.tokens ? c.length + tok + 1 - c.tokens : 0u;
+        const uint32_t low = a.window != 0 && past > a.window ? past - a.window : 0u;
+        const size_t row_at = (static_cast<size_t>(c.q0 + tok) * a.q_heads + head) * D;
+        const bool wave_live = wave * 32 < span.rows;
+        // of the wave's first and last row
+        const uint32_t past_a = __builtin_amdgcn_readfirstlane(past), low_a = __builtin_amdgcn_readfirstlane(low);
+        const uint32_t past_z = __builtin_amdgcn_readlane(past, 31), low_z = __builtin_amdgcn_readlane(low, 31);
+
+        half8 qf[NQ];
+        with_type(a.q_dtype, [&](auto t) __attribute__((always_inline)) {
+#pragma unroll
+            for (uint32_t k = 0; k < NQ; ++k) qf[k] = load_query<decltype(t)>(a.q, row_at + 16 * k + 8 * hh);
+        });
+        if (a.negate)
+#pragma unroll
+            for (uint32_t k = 0; k < NQ; ++k) qf[k] = -qf[k];
+
+        // Row (page * kv_heads + head) * page_tokens + slot of the i-th step's first key.
+        auto row_of = [&](uint32_t i) __attribute__((always_inline)) {
+            const uint32_t tok0 = uniform(span.vis.step(i) * kChunk);
+            uint32_t page = 0, tp = tok0;
+            if (geo.layout == MIIKV_LAYOUT_PAGED) {
+                const uint32_t e = uniform(tok0 / geo.page_tokens);
+                tp = tok0 - e * geo.page_tokens;
+                page = min(static_cast<uint32_t>(scalar_load(geo.table + static_cast<size_t>(b) * geo.table_stride + e)),
+                           geo.num_pages - 1);
+            }
+            return (static_cast<size_t>(page) * geo.kv_heads + h) * geo.page_tokens + tp;
+        };
+        // A step's bytes into its place in the ring, without registers: the waves share the KiB of
+        // codes, and each copies an eighth of the scales.
+        auto fetch = [&](uint32_t i) __attribute__((always_inline)) {
+            const size_t kv = row_of(i);
+            const uint32_t to = lds_offset(s_raw) + i % Lds::bufs * Lds::raw;
+            const char* k = reinterpret_cast<const char*>(geo.k_codes) + kv * (D * KE);
+            const char* v = reinterpret_cast<const char*>(geo.v_codes) + kv * (D * VE);
+#pragma unroll
+            for (uint32_t x = 0; x * kChunkWaves * 1024 < Lds::k_bytes + Lds::v_bytes; ++x) {
+                const uint32_t at = (wave + x * kChunkWaves) * 1024;
+                if (at < Lds::k_bytes + Lds::v_bytes)  // (12 KiB in the mixed modes at D = 128)
+                    copy_to_lds((at < Lds::k_bytes ? k + at : v + (at - Lds::k_bytes)) + lane * 16, to + at);
+            }
+            if constexpr (!(KF16 && VF16)) {
+                constexpr uint32_t kEach = 2 * Lds::scale_bytes / kChunkWaves;  // of K's, then of V's
+                const uint32_t at = wave * kEach;
+                const bool of_k = at < Lds::scale_bytes;
+                if (lane < kEach / 16 && !(of_k ? KF16 : VF16))
+                    copy_to_lds(reinterpret_cast<const char*>(of_k ? geo.k_scales + kv * NB : geo.v_scales + kv * NB) +
+                                    (of_k ? at : at - Lds::scale_bytes) + lane * 16,
+                                to + Lds::k_bytes + Lds::v_bytes + at);
+            }
+        };
+        // Keys of the step that no row of the item sees may hold anything: their values are zeroed.
+        auto unseen = [&](uint32_t t) __attribute__((always_inline)) {
+            return (t >= span.past) | ((t < span.vis.lo) & (t >= a.sinks));
+        };
+        // V's scales, two blocks of one key per thread, in the order of V's units.
+        auto order_scales = [&](uint32_t i) __attribute__((always_inline)) {
+            if (!VF16 && tid < 16 * NB) {
+                const uint32_t key = tid / (NB / 2), blk = tid % (NB / 2) * 2;
+                uint32_t w = *reinterpret_cast<const uint32_t*>(s_raw + i % Lds::bufs * Lds::raw + Lds::k_bytes + Lds::v_bytes +
+                                                                Lds::scale_bytes + tid * 4);
+                if (unseen(span.vis.step(i) * kChunk + key)) w = 0;
+                _Float16* to = s_vsc + (i & 1) * D + blk * 32 + ((key >> 2) & 3) * 8 + (key >> 4) * 4 + (key & 3);
+                to[0] = tile_scale(static_cast<uint16_t>(w & 0xffffu));
+                to[32] = tile_scale(static_cast<uint16_t>(w >> 16));
+            }
+        };
+        // A step's codes to fp16: each thread 16 codes of K and / or of V.
+        constexpr bool kBoth = D == 256;
+        auto convert = [&](uint32_t i) __attribute__((always_inline)) {
+            const uint32_t idx = kBoth ? tid : tid & 255u;
+            const uint8_t* raw = s_raw + i % Lds::bufs * Lds::raw;
+            half8* tile = s_tile + (i & 1) * Lds::units;
+            if (kBoth || tid < 256) {
+                // key 16 T + m, dims 64 c + 8 g and 64 c + 32 + 8 g
+                const uint32_t T = idx / D, c = idx / 64 % (D / 64), g = idx / 16 % 4, m = idx % 16;
+                half8* to = tile + (8 * c + g) * kChunk + 16 * T + m;
+                const uint4* from = reinterpret_cast<const uint4*>(raw) + idx * KE;
+                if constexpr (KF16) {
+                    to[0] = __builtin_bit_cast(half8, from[0]);
+                    to[4 * kChunk] = __builtin_bit_cast(half8, from[1]);
+                } else {
+                    const uint4 w = from[0];
+                    const uint32_t f = *reinterpret_cast<const uint32_t*>(raw + Lds::k_bytes + Lds::v_bytes + ((16 * T + m) * NB + 2 * c) * 2);
+                    to[0] = codes8_to_half8(w.x, w.y) * tile_scale(static_cast<uint16_t>(f & 0xffffu));
+                    to[4 * kChunk] = codes8_to_half8(w.z, w.w) * tile_scale(static_cast<uint16_t>(f >> 16));
+                }
+            }
+            if (kBoth || tid >= 256) {
+                // dim d, keys of units 2x and 2x + 1
+                const uint32_t d = idx / 2, x = idx % 2;
+                half8* to = tile + Lds::k_units + 2 * x * Lds::v_row + d;
+                const uint4* from = reinterpret_cast<const uint4*>(raw + Lds::k_bytes) + idx * VE;
+                if constexpr (VF16) {
+                    half8 v[2] = {__builtin_bit_cast(half8, from[0]), __builtin_bit_cast(half8, from[VF16 ? 1 : 0])};
+                    const uint32_t tok0 = uniform(span.vis.step(i) * kChunk);
+                    if (tok0 + kChunk > span.past || (tok0 < span.vis.lo && tok0 + kChunk > a.sinks)) {
+#pragma unroll
+                        for (uint32_t u = 0; u < 2; ++u)
+#pragma unroll
+                            for (uint32_t y = 0; y < 8; ++y)
+                                v[u][y] = unseen(tok0 + 16 * (y / 4) + 4 * (2 * x + u) + y % 4) ? static_cast<_Float16>(0.0f) : v[u][y];
+                    }
+                    to[0] = v[0];
+                    to[Lds::v_row] = v[1];
+                } else {
+                    const uint4 w = from[0];
+                    const half8* f = reinterpret_cast<const half8*>(s_vsc + (i & 1) * D + d / 32 * 32 + 16 * x);
+                    to[0] = codes8_to_half8(w.x, w.y) * f[0];
+                    to[Lds::v_row] = codes8_to_half8(w.z, w.w) * f[1];
+                }
+            }
+        };
+
+        float m_run = -INFINITY, l_run = 0.0f;
+        float16v O[NB];
+#pragma unroll
+        for (uint32_t mt = 0; mt < NB; ++mt)
+#pragma unroll
+            for (uint32_t x = 0; x < 16; ++x) O[mt][x] = 0.0f;
+
+        if (s0 < s1) {
+            lds_barrier();  // the previous item's tiles and ring have been read
+            for (uint32_t i = s0; i < min(s0 + Lds::bufs, s1); ++i) fetch(i);
+            wait_vmem();
+            lds_barrier();
+            order_scales(s0);
+            if (s0 + 1 < s1) order_scales(s0 + 1);
+            lds_barrier();
+            convert(s0);
+        }
+        for (uint32_t s = s0; s < s1; ++s) {
+            // The step that is `landed` ahead is whole in the ring, of every wave's copies.
+            if (s != s0) {
+                if (KF16 == VF16 && s + Lds::bufs - 1 < s1) wait_vmem_le<(Lds::bufs - 1 - Lds::landed) * Lds::ops>();
+                else wait_vmem();
+            }
+            lds_barrier();
+            if (s + Lds::bufs < s1) fetch(s + Lds::bufs);  // where step s was, which is a tile now
+            if (s + 2 < s1) order_scales(s + 2);
+            if (s + 1 < s1) convert(s + 1);
+
+            const uint32_t tok0 = uniform(span.vis.step(s) * kChunk);
+            // Nothing of the step is seen by this wave's rows (wave-uniform)?
+            if (!wave_live || tok0 >= past_z || (a.window != 0 && tok0 + kChunk <= low_a && tok0 >= a.sinks)) continue;
+            const bool whole = tok0 + kChunk <= past_a && (a.window == 0 || tok0 + kChunk <= a.sinks || tok0 >= low_z);
+            const half8* tile = s_tile + (s & 1) * Lds::units;
+            float16v S;
+#pragma unroll
+            for (uint32_t x = 0; x < 16; ++x) S[x] = 0.0f;
+            mfma_pairs<NQ>(tile + hh * kChunk + n, 2 * kChunk, [&](uint32_t k, half8 f) __attribute__((always_inline)) {
+                S = mfma_32x32x16(f, qf[k], S);
+            });
+            if (!whole) {
+#pragma unroll
+                for (uint32_t x = 0; x < 16; ++x) {
+                    const uint32_t t = tok0 + 8 * (x / 4) + 4 * hh + x % 4;
+                    S[x] = (t >= past) | ((t < low) & (t >= a.sinks)) ? -INFINITY : S[x];
+                }
+            }
+            float top = S[0];
+#pragma unroll
+            for (uint32_t x = 1; x < 16; ++x) top = fmaxf(top, S[x]);
+            top = swap32_reduce(top, MaxOp{}) * a.scale_log2;
+            if (__any(top > m_run + kSlack)) {
+                const float to = fmaxf(m_run, top);
+                const float f = m_run == -INFINITY ? 0.0f : exp2_fast(m_run - to);
+                m_run = to;
+                l_run *= f;
+#pragma unroll
+                for (uint32_t mt = 0; mt < NB; ++mt) O[mt] *= f;
+            }
+            const float use = m_run == -INFINITY ? 0.0f : m_run;
+            half8 P[2];
+#pragma unroll
+            for (uint32_t x = 0; x < 16; ++x) {
+                const float p = exp2_fast(fmaf(S[x], a.scale_log2, -use));
+                l_run += p;
+                P[x / 4 % 2][x % 4 + x / 8 * 4] = static_cast<_Float16>(p);
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < 2; ++u)
+                mfma_pairs<NB>(tile + Lds::k_units + (2 * u + hh) * Lds::v_row + n, kChunk, [&](uint32_t mt, half8 f) __attribute__((always_inline)) {
+                    O[mt] = mfma_32x32x16(f, P[u], O[mt]);
+                });
+        }
+        l_run = swap32_reduce(l_run, AddOp{});
+        const float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;  // a token that sees no key: zeros
+        if (s1 - s0 == steps) {
+            if (row_live)
+                with_type(a.out_dtype, [&](auto t) __attribute__((always_inline)) {
+#pragma unroll
+                    for (uint32_t mt = 0; mt < NB; ++mt)
+#pragma unroll
+                        for (uint32_t x = 0; x < 16; x += 4)
+                            store4<decltype(t)>(a.out, row_at + 32 * mt + 2 * x + 4 * hh,
+                                                make_float4(O[mt][x] * inv, O[mt][x + 1] * inv, O[mt][x + 2] * inv, O[mt][x + 3] * inv));
+                });
+        } else if (row_live) {
+            const size_t rec = (static_cast<size_t>(2 * part + (first < begin ? 0u : 1u)) * kRows + r);
+#pragma unroll
+            for (uint32_t mt = 0; mt < NB; ++mt)
+#pragma unroll
+                for (uint32_t x = 0; x < 4; ++x) {
+                    half4 o;
+#pragma unroll
+                    for (uint32_t y = 0; y < 4; ++y) o[y] = static_cast<_Float16>(O[mt][4 * x + y] * inv);
+                    *reinterpret_cast<half4*>(a.rec_o + rec * D + 32 * mt + 8 * x + 4 * hh) = o;
+                }
+            if (hh == 0) a.rec_ml[rec] = make_float2(m_run, l_run);
+        }
+    }
+}
+
+// Merge of the items that were cut: workgroup (item, kv head, 32 rows), 8 threads per row.
+constexpr uint32_t kMergeRows = 32;
+template <uint32_t D>
+__global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs a) {
+    const uint32_t i = blockIdx.x / (kRows / kMergeRows), h = blockIdx.y;
+    if (i >= a.head[0]) return;
+    const ChunkItem it = a.items[i];
+    const uint32_t units = a.head[1], quota = a.head[2];
+    const uint32_t first = h * units + it.start + kItemCost;
+    if (it.steps == 0) return;
+    const uint32_t w0 = first / quota, w1 = (first + it.steps - 1) / quota;
+    if (w0 == w1) return;  // written whole
+    const uint32_t r = blockIdx.x % (kRows / kMergeRows) * kMergeRows + threadIdx.x / 8;
+    const Chunk c = chunk_of(a, it.b);
+    if (it.rows0 + r >= c.tokens * a.group) return;
+    const uint32_t tok = (it.rows0 + r) / a.group, head = h * a.group + (it.rows0 + r) % a.group;
+    float m = -INFINITY;
+    for (uint32_t w = w0; w <= w1; ++w) {
+        const size_t rec = static_cast<size_t>(2 * w + (first < w * quota ? 0u : 1u)) * kRows + r;
+        m = fmaxf(m, a.rec_ml[rec].x);
+    }
+    constexpr uint32_t kPer = D / 64;  // groups of 8 values per thread
+    float acc[kPer][8] = {};
+    float sum = 0.0f;
+    for (uint32_t w = w0; w <= w1; ++w) {
+        const size_t rec = static_cast<size_t>(2 * w + (first < w * quota ? 0u : 1u)) * kRows + r;
+        const float2 ml = a.rec_ml[rec];
+        const float f = ml.x == -INFINITY ? 0.0f : ml.y * exp2_fast(ml.x - m);
+        sum += f;
+#pragma unroll
+        for (uint32_t k = 0; k < kPer; ++k) {
+            const half8 o = *reinterpret_cast<const half8*>(a.rec_o + rec * D + 64 * k + 8 * (threadIdx.x % 8));
+#pragma unroll
+            for (uint32_t x = 0; x < 8; ++x) acc[k][x] = fmaf(static_cast<float>(o[x]), f, acc[k][x]);
+        }
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    const size_t at = (static_cast<size_t>(c.q0 + tok) * a.q_heads + head) * D + 8 * (threadIdx.x % 8);
+    with_type(a.out_dtype, [&](auto t) __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t k = 0; k < kPer; ++k)
+#pragma unroll
+            for (uint32_t x = 0; x < 8; x += 4)
+                store4<decltype(t)>(a.out, at + 64 * k + x, make_float4(acc[k][x] * inv, acc[k][x + 1] * inv, acc[k][x + 2] * inv, acc[k][x + 3] * inv));
+    });
+}
+
+uint64_t up256(uint64_t x) { return (x + 255) / 256 * 256; }
+
+uint32_t chunk_lds_bytes(uint32_t D, bool kf, bool vf) {
+    if (D == 128)
+        return kf ? (vf ? ChunkLds<128, true, true>::bytes : ChunkLds<128, true, false>::bytes)
+                  : (vf ? ChunkLds<128, false, true>::bytes : ChunkLds<128, false, false>::bytes);
+    return kf ? (vf ? ChunkLds<256, true, true>::bytes : ChunkLds<256, true, false>::bytes)
+              : (vf ? ChunkLds<256, false, true>::bytes : ChunkLds<256, false, false>::bytes);
+}
+
+struct ChunkPlan {
+    uint64_t items;  // of one kv head, at most
+    uint32_t parts;
+    size_t lds;
+    uint64_t item_bytes, o_bytes, ml_bytes;
+    uint64_t bytes() const { return 256 + item_bytes + o_bytes + ml_bytes; }
+};
+
+// Sizes and the plan's bounds; a status.
+int chunk_plan(const miikv_view* v, uint32_t q_heads, uint32_t batch, uint32_t total_tokens, uint32_t max_tokens,
+               uint32_t max_context, uint32_t window, uint32_t sinks, ChunkPlan& p) {
+    const int st = validate_view(v);
+    if (st != MIIKV_OK) return st;
+    if (batch == 0 || total_tokens == 0 || max_tokens == 0 || q_heads == 0 || q_heads % v->kv_heads != 0) return MIIKV_EINVAL;
+    if (max_context == 0 || max_context > view_seq_capacity(v) || max_context > 0x7fffffffu) return MIIKV_EINVAL;
+    if (max_tokens > total_tokens || max_tokens > max_context) return MIIKV_EINVAL;
+    if (v->layout == MIIKV_LAYOUT_CONTIGUOUS && batch != 1) return MIIKV_EINVAL;
+    const uint64_t rows = static_cast<uint64_t>(total_tokens) * (q_heads / v->kv_heads);
+    if (rows > 0x7fffffffu || batch > 65535u || v->kv_heads > 65535u) return MIIKV_EUNSUPPORTED;
+    // every sequence's last item may be a part of one
+    p.items = std::min<uint64_t>(rows / kRows + batch, rows);
+    const uint64_t most = kItemCost + most_visible_steps(max_context, max_tokens, window, sinks);
+    const uint64_t axis = p.items * most * v->kv_heads;
+    if (axis / v->kv_heads / most != p.items || axis > 0xf0000000u) return MIIKV_EUNSUPPORTED;  // 32-bit places on the axis
+    p.parts = static_cast<uint32_t>(std::min<uint64_t>(kMaxParts, (axis + kMinUnits - 1) / kMinUnits));
+    const uint32_t D = v->head_dim;
+    p.lds = chunk_lds_bytes(D, mode_k_f16(v->quant_mode), mode_v_f16(v->quant_mode)) +
+            (static_cast<size_t>(batch) + 1 + p.items + 1) * sizeof(uint32_t);
+    if (p.lds > 159 * 1024) return MIIKV_EUNSUPPORTED;
+    p.item_bytes = up256(p.items * sizeof(ChunkItem));
+    p.o_bytes = up256(2ull * p.parts * kRows * D * sizeof(uint16_t));
+    p.ml_bytes = up256(2ull * p.parts * kRows * 2 * sizeof(float));
+    return MIIKV_OK;
+}
+
+template <uint32_t D>
+int launch_chunk(const ChunkArgs& a, const ChunkPlan& p, bool kf, bool vf, hipStream_t s) {
+    const dim3 grid((p.parts + 7) / 8 * 8);
+    const auto go = [&](auto k, auto v) {
+        hipLaunchKernelGGL((chunk_kernel<D, decltype(k)::value, decltype(v)::value>), grid, dim3(kChunkThreads), p.lds, s, a);
+    };
+    const auto with_v = [&](auto k) { vf ? go(k, std::true_type{}) : go(k, std::false_type{}); };
+    kf ? with_v(std::true_type{}) : with_v(std::false_type{});
+    hipLaunchKernelGGL((chunk_merge_kernel<D>), dim3(static_cast<uint32_t>(p.items) * (kRows / kMergeRows), a.g.kv_heads), dim3(256), 0, s, a);
+    return hip_status(hipGetLastError());
+}
+
+}  // namespace
+}  // namespace miikv
+
+using namespace miikv;
+
+extern "C" uint64_t miikv_chunk_workspace_bytes(const miikv_view* view, uint32_t q_heads, uint32_t batch,
+                                                uint32_t total_tokens, uint32_t max_tokens, uint32_t max_context,
+                                                uint32_t window, uint32_t sinks) {
+    ChunkPlan p{};
+    if (window >= max_context) window = 0;
+    if (chunk_plan(view, q_heads, batch, total_tokens, max_tokens, max_context, window, std::min(sinks, max_context), p) != MIIKV_OK)
+        return 0;
+    return p.bytes();
+}
+
+extern "C" miikv_status miikv_chunk_attn(const miikv_view* view, const void* q, uint32_t q_dtype, uint32_t q_heads,
+                                         float scale, uint32_t batch, uint32_t total_tokens, const uint32_t* d_offsets,
+                                         const uint32_t* d_lengths, uint32_t max_tokens, uint32_t max_context,
+                                         uint32_t window, uint32_t sinks, void* out, uint32_t out_dtype, void* workspace,
+                                         uint64_t workspace_bytes, void* stream) {
+    ChunkPlan p{};
+    if (window >= max_context) window = 0;  // hides nothing
+    sinks = std::min(sinks, max_context);
+    const int st = chunk_plan(view, q_heads, batch, total_tokens, max_tokens, max_context, window, sinks, p);
+    if (st != MIIKV_OK) return st;
+    if (q == nullptr || out == nullptr || d_offsets == nullptr || d_lengths == nullptr || !std::isfinite(scale) ||
+        q_dtype > MIIKV_DTYPE_BF16 || out_dtype > MIIKV_DTYPE_BF16)
+        return MIIKV_EINVAL;
+    if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || !aligned16(view->k_codes) || !aligned16(view->v_codes) ||
+        !aligned16(view->k_scales) || !aligned16(view->v_scales))
+        return MIIKV_EINVAL;
+    if (workspace == nullptr || workspace_bytes < p.bytes()) return MIIKV_EWORKSPACE;
+    ChunkArgs a{};
+    a.g = make_geo(*view);
+    a.q = q;
+    a.q_dtype = q_dtype;
+    a.q_heads = q_heads;
+    a.group = q_heads / view->kv_heads;
+    a.scale_log2 = std::max(std::fabs(scale) * kLog2eF, 1e-30f);  // (0 times a hidden key's -inf would be NaN)
+    a.negate = scale < 0.0f ? 1u : 0u;
+    a.batch = batch;
+    a.total_tokens = total_tokens;
+    a.max_tokens = max_tokens;
+    a.max_context = max_context;
+    a.window = window;
+    a.sinks = sinks;
+    a.offsets = d_offsets;
+    a.lengths = d_lengths;
+    a.out = out;
+    a.out_dtype = out_dtype;
+    a.most_items = static_cast<uint32_t>(p.items);
+    a.parts = p.parts;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    a.head = reinterpret_cast<uint32_t*>(ws);
+    a.items = reinterpret_cast<ChunkItem*>(ws + 256);
+    a.rec_o = reinterpret_cast<_Float16*>(ws + 256 + p.item_bytes);
+    a.rec_ml = reinterpret_cast<float2*>(ws + 256 + p.item_bytes + p.o_bytes);
+    const bool kf = mode_k_f16(view->quant_mode), vf = mode_v_f16(view->quant_mode);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return view->head_dim == 128 ? launch_chunk<128>(a, p, kf, vf, s) : launch_chunk<256>(a, p, kf, vf, s);
+}

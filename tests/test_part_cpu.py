@@ -176,3 +176,58 @@ def test_python_refusals():
                 dict(budget=16, new_lengths=torch.zeros(1))):
         with pytest.raises(ValueError):
             m.evict(cache, w, lens, **bad)
+
+
+def _chunk(lib, v, **over):
+    a = dict(q=P, qt=2, heads=32, scale=F, batch=3, total=100, off=P, lengths=P, most_tokens=64, most=4096, window=128, sinks=4,
+             out=P, ot=2, ws=P, bytes=1 << 40)
+    a.update(over)
+    return lib.miikv_chunk_attn(None if v is None else ctypes.byref(v), a["q"], a["qt"], a["heads"], a["scale"], a["batch"],
+                                a["total"], a["off"], a["lengths"], a["most_tokens"], a["most"], a["window"], a["sinks"],
+                                a["out"], a["ot"], a["ws"], a["bytes"], None)
+
+
+@pytest.mark.parametrize("over,status", [
+    ({"q": None}, 1), ({"out": None}, 1), ({"off": None}, 1), ({"lengths": None}, 1), ({"qt": 3}, 1), ({"ot": 3}, 1),
+    ({"heads": 30}, 1), ({"heads": 0}, 1), ({"scale": ctypes.c_float(float("inf"))}, 1), ({"batch": 0}, 1), ({"total": 0}, 1),
+    ({"most_tokens": 0}, 1), ({"most_tokens": 101}, 1), ({"total": 9000, "most_tokens": 5000}, 1), ({"most": 0}, 1),
+    ({"most": 4097}, 1), ({"ws": None}, 3), ({"bytes": 256}, 3), ({"q": ctypes.c_void_p(0x10008)}, 1),
+    ({"out": ctypes.c_void_p(0x10004)}, 1), ({"ws": ctypes.c_void_p(0x10008)}, 1),
+    ({"batch": 70000}, 2), ({"batch": 60000}, 2), ({"total": 0x7fffffff}, 2),
+])
+def test_chunk_refuses(over, status):
+    L = _lib()
+    assert _chunk(L.lib(), _paged(), **over) == status
+    assert _chunk(L.lib(), None) == L.MIIKV_EINVAL
+    assert _chunk(L.lib(), _view(), batch=2) == L.MIIKV_EINVAL  # a contiguous cache holds one sequence
+
+
+def test_chunk_workspace_sizes():
+    L = _lib()
+    lib = L.lib()
+    v = _paged()
+    r = ctypes.byref(v)
+    need = lib.miikv_chunk_workspace_bytes(r, 32, 3, 100, 64, 4096, 128, 4)
+    assert need > 0 and _chunk(lib, v, bytes=need - 1) == L.MIIKV_EWORKSPACE
+    assert lib.miikv_chunk_workspace_bytes(r, 32, 3, 100, 64, 4096, 0xffffffff, 0xffffffff) == \
+        lib.miikv_chunk_workspace_bytes(r, 32, 3, 100, 64, 4096, 0, 0)
+    for bad in ((30, 3, 100, 64, 4096), (32, 0, 100, 64, 4096), (32, 3, 0, 1, 4096), (32, 3, 100, 101, 4096), (32, 3, 100, 64, 4097)):
+        assert lib.miikv_chunk_workspace_bytes(r, *bad, 0, 0) == 0
+
+
+def test_chunk_python_refusals():
+    import torch
+
+    import miinfer_amd as m
+    planes = [torch.zeros(2 * 8 * 64 * 128, dtype=torch.float16) for _ in range(2)]
+    cache = m.KvCache.from_planes(8, 128, *planes, page_tokens=64, block_table=torch.zeros((1, 2), dtype=torch.int32))
+    q = torch.zeros((4, 32, 128), dtype=torch.bfloat16)
+    off, lens = torch.tensor([0, 4], dtype=torch.int32), torch.tensor([9], dtype=torch.int32)
+    with pytest.raises(ValueError, match="GPU"):
+        m.chunk_attention(cache, q, off, lens)
+    for args, kw in (((q.double(), off, lens), {}), ((q[:, :, ::2], off, lens), {}), ((q, off[:1], lens), {}),
+                     ((q, off.long(), lens), {}), ((q, off, lens), {"out": q.int()}), ((q, off, lens), {"out": q[:3]}),
+                     ((q, off, lens), {"window": -1}), ((q, off, lens), {"max_tokens": 0}),
+                     ((q, torch.tensor([0, 1, 4], dtype=torch.int32), torch.ones(2, dtype=torch.int32)), {})):
+        with pytest.raises(ValueError):
+            m.chunk_attention(cache, *args, **kw)
