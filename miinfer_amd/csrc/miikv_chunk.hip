@@ -66,6 +66,8 @@ struct ChunkArgs {
     uint32_t out_dtype;
     uint32_t most_items;  // of one kv head
     uint32_t parts;
+    uint32_t page_steps;  // steps per page, and for small ones 2^32 / page_steps, rounded up
+    uint32_t page_magic;
     // workspace
     uint32_t* head;      // [0] items of one kv head, [1] units of one kv head, [2] units per part
     ChunkItem* items;    // [most_items]
@@ -101,6 +103,11 @@ __device__ __forceinline__ Chunk chunk_of_uniform(const ChunkArgs& a, uint32_t b
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+
+__device__ __forceinline__ const char* uniform_ptr(const char* p) {
+    const uint64_t x = reinterpret_cast<uint64_t>(p);
+    return reinterpret_cast<const char*>(static_cast<uint64_t>(uniform(static_cast<uint32_t>(x >> 32))) << 32 | uniform(static_cast<uint32_t>(x)));
+}
 
 // What the rows rows0 .. of a chunk see together: the context of the last of them, their
 // tokens and the steps.
@@ -145,23 +152,18 @@ __device__ __forceinline__ uint32_t scan_threads(uint32_t x, uint32_t* s_wave, u
 __device__ __forceinline__ float16v mfma_32x32x16(half8 a, half8 b, float16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
-// `use`(c, t[c * stride]) for c < N; the next pair of fragments is on its way from LDS while
-// a pair's MFMAs run.
-template <uint32_t N, typename F>
-__device__ __forceinline__ void mfma_pairs(const half8* t, uint32_t stride, F use) {
-    half8 f[2][2] = {{t[0], t[stride]}, {}};
-#pragma unroll
-    for (uint32_t c = 0; c < N; c += 2) {
-        const uint32_t k = (c / 2) & 1;
-        if (c + 2 < N) {
-            f[k ^ 1][0] = t[(c + 2) * stride];
-            f[k ^ 1][1] = t[(c + 3) * stride];
-        }
-        __builtin_amdgcn_sched_barrier(0);  // the scheduler would move the reads to their use, or all of them up here
-        use(c, f[k][0]);
-        use(c + 1, f[k][1]);
-        __builtin_amdgcn_sched_barrier(0);
-    }
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+    return r;
+}
+// 16 bytes per lane from `base` + `off` to LDS at `lds` + 16 * lane (`base` and `lds` wave-uniform;
+// counted by the caller, as copy_to_lds).
+__device__ __forceinline__ void copy_to_lds_from(const char* base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(uniform_ptr(base))
+                 : "memory", "m0");
 }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -194,10 +196,10 @@ __device__ __forceinline__ half8 load_query(const void* q, size_t at) {
     }
 }
 
-// A block scale of a tile: 128 * 511.75 = 65504 is the largest that leaves every code finite.
+// Block scales of a tile: 128 * 511.75 = 65504 is the largest that leaves every code finite.
 // (Larger ones stand for blocks within 0.8% of fp16's maximum.)
-__device__ __forceinline__ _Float16 tile_scale(uint16_t bits) {
-    return __builtin_elementwise_min(__builtin_bit_cast(_Float16, bits), static_cast<_Float16>(511.75f));
+__device__ __forceinline__ half2v tile_scales(half2v s) {
+    return __builtin_elementwise_min(s, half2v{static_cast<_Float16>(511.75f), static_cast<_Float16>(511.75f)});
 }
 
 // LDS of chunk_kernel: two fp16 tiles of a step, K units [D / 8][32 keys] and V units [4][D + 4]
@@ -219,6 +221,9 @@ struct ChunkLds {
     static constexpr uint32_t bufs = D == 128 || !(KF16 || VF16) ? 4 : (KF16 && VF16 ? 2 : 3);
     static constexpr uint32_t landed = VF16 ? 1 : 2;
     static constexpr uint32_t ops = (k_bytes + v_bytes) / 1024 / kChunkWaves + (KF16 && VF16 ? 0 : 1);
+    // Whether the waves of a SIMD take turns at the matrix and the vector unit: where the ring holds
+    // four steps.
+    static constexpr bool turns = !KF16 && !VF16;
     static constexpr uint32_t vsc_bytes = 2 * 2 * D;  // V's scales of two steps in the order of its units
     static constexpr uint32_t bytes = 2 * units * 16 + bufs * raw + vsc_bytes;
 };
@@ -228,6 +233,7 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
     constexpr uint32_t NB = D / 32;
     constexpr uint32_t NQ = D / 16;  // K-axis chunks of the first product
     constexpr uint32_t KE = KF16 ? 2 : 1, VE = VF16 ? 2 : 1;
+    constexpr uint32_t kAhead = D == 128 ? 8 : 4;  // fragments read ahead of their MFMAs
     using Lds = ChunkLds<D, KF16, VF16>;
     extern __shared__ __align__(16) uint8_t lds[];
     half8* const s_tile = reinterpret_cast<half8*>(lds);  // two tiles
@@ -298,28 +304,25 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
     if (static_cast<uint64_t>(part) * quota >= axis) return;
     const uint32_t begin = part * quota, end = axis - begin < quota ? axis : begin + quota;
     uint32_t at = begin;
-
-    while (at < end) {
-        const uint32_t h = uniform(at / units);
-        const uint32_t in_head = at - h * units;
-        uint32_t i = 0;
-        {
-            uint32_t hi = items;
-            while (hi - i > 1) {
-                const uint32_t mid = (i + hi) / 2;
-                if (uniform(s_start[mid]) <= in_head) i = mid;
-                else hi = mid;
-            }
+    uint32_t h = uniform(at / units);
+    uint32_t i = 0, b = 0;  // the item that holds `at`, and its sequence
+    for (uint32_t hi = items; hi - i > 1;) {
+        const uint32_t mid = (i + hi) / 2;
+        if (uniform(s_start[mid]) <= at - h * units) i = mid;
+        else hi = mid;
+    }
+    for (uint32_t hi = a.batch; hi - b > 1;) {
+        const uint32_t mid = (b + hi) / 2;
+        if (uniform(s_first[mid]) <= i) b = mid;
+        else hi = mid;
+    }
+    for (; at < end; ++i) {
+        if (i == items) {  // the next kv head's first
+            ++h;
+            i = 0;
+            b = 0;
         }
-        uint32_t b = 0;
-        {
-            uint32_t hi = a.batch;
-            while (hi - b > 1) {
-                const uint32_t mid = (b + hi) / 2;
-                if (uniform(s_first[mid]) <= i) b = mid;
-                else hi = mid;
-            }
-        }
+        while (uniform(s_first[b + 1]) <= i) ++b;
         const uint32_t start = h * units + uniform(s_start[i]), stop = h * units + uniform(s_start[i + 1]);
         const Chunk c = chunk_of_uniform(a, b);
         const uint32_t rows0 = (i - uniform(s_first[b])) * kRows;
@@ -348,73 +351,102 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
         const uint32_t past_a = __builtin_amdgcn_readfirstlane(past), low_a = __builtin_amdgcn_readfirstlane(low);
         const uint32_t past_z = __builtin_amdgcn_readlane(past, 31), low_z = __builtin_amdgcn_readlane(low, 31);
 
-        half8 qf[NQ];
-        with_type(a.q_dtype, [&](auto t) __attribute__((always_inline)) {
-#pragma unroll
-            for (uint32_t k = 0; k < NQ; ++k) qf[k] = load_query<decltype(t)>(a.q, row_at + 16 * k + 8 * hh);
-        });
-        if (a.negate)
-#pragma unroll
-            for (uint32_t k = 0; k < NQ; ++k) qf[k] = -qf[k];
-
-        // Row (page * kv_heads + head) * page_tokens + slot of the i-th step's first key.
-        auto row_of = [&](uint32_t i) __attribute__((always_inline)) {
-            const uint32_t tok0 = uniform(span.vis.step(i) * kChunk);
-            uint32_t page = 0, tp = tok0;
-            if (geo.layout == MIIKV_LAYOUT_PAGED) {
-                const uint32_t e = uniform(tok0 / geo.page_tokens);
-                tp = tok0 - e * geo.page_tokens;
-                page = min(static_cast<uint32_t>(scalar_load(geo.table + static_cast<size_t>(b) * geo.table_stride + e)),
-                           geo.num_pages - 1);
-            }
-            return (static_cast<size_t>(page) * geo.kv_heads + h) * geo.page_tokens + tp;
+        // The thread's number, at D = 256 made anew at each use: what is derived from it is then not
+        // kept in registers through the loop (which has none left there).
+        auto here = [&]() __attribute__((always_inline)) {
+            uint32_t t = tid;
+            if constexpr (D == 256) asm volatile("" : "+v"(t));
+            return t;
         };
-        // A step's bytes into its place in the ring, without registers: the waves share the KiB of
-        // codes, and each copies an eighth of the scales.
-        auto fetch = [&](uint32_t i) __attribute__((always_inline)) {
-            const size_t kv = row_of(i);
-            const uint32_t to = lds_offset(s_raw) + i % Lds::bufs * Lds::raw;
-            const char* k = reinterpret_cast<const char*>(geo.k_codes) + kv * (D * KE);
-            const char* v = reinterpret_cast<const char*>(geo.v_codes) + kv * (D * VE);
+        // Steps go into the ring one after another, by copies that pass no registers: the waves share
+        // the KiB of codes, and each copies an eighth of the scales.  A wave keeps the addresses of
+        // its pieces and steps them on; at a page's end (and where the steps of the first tokens end) they
+        // are made anew, from 64 entries of the block table held by the lanes.
+        constexpr uint32_t kPieces = (Lds::k_bytes + Lds::v_bytes + 1024 * kChunkWaves - 1) / 1024 / kChunkWaves;
+        constexpr uint32_t kScalePiece = 2 * Lds::scale_bytes / kChunkWaves;  // of K's, then of V's
+        const bool scale_of_k = wave < kChunkWaves / 2;
+        const char* src[kPieces];
+        const char* src_scale = nullptr;
+        uint32_t next = s0, run_left = 0;
+        uint32_t tab = 0, tab0 = 0x80000000u;  // (none yet)
+        auto locate = [&]() __attribute__((always_inline)) {
+            const uint32_t st = uniform(span.vis.step(next));
+            uint32_t page = 0, slot = st;
+            run_left = 0x7fffffffu;
+            if (geo.layout == MIIKV_LAYOUT_PAGED) {
+                const uint32_t e = a.page_magic != 0 ? __umulhi(st, a.page_magic) : uniform(st / a.page_steps);
+                if (e - tab0 >= 64u) {
+                    tab0 = e;
+                    // (waited for here, in asm: the compiler would wait for every copy at each use)
+                    const int32_t* from = geo.table + static_cast<size_t>(b) * geo.table_stride + min(e + lane, geo.table_stride - 1);
+                    asm volatile("global_load_dword %0, %1, off\n\ts_waitcnt vmcnt(0)" : "=&v"(tab) : "v"(from) : "memory");
+                    tab = min(tab, geo.num_pages - 1);
+                }
+                page = __builtin_amdgcn_readlane(tab, e - tab0);
+                slot = st - e * a.page_steps;
+                run_left = a.page_steps - slot;
+            }
+            if (next < span.vis.head) run_left = min(run_left, span.vis.head - next);
+            const size_t kv = (static_cast<size_t>(page) * geo.kv_heads + h) * geo.page_tokens + slot * kChunk;
 #pragma unroll
-            for (uint32_t x = 0; x * kChunkWaves * 1024 < Lds::k_bytes + Lds::v_bytes; ++x) {
+            for (uint32_t x = 0; x < kPieces; ++x) {
+                const uint32_t at = (wave + x * kChunkWaves) * 1024;
+                src[x] = uniform_ptr(at < Lds::k_bytes ? reinterpret_cast<const char*>(geo.k_codes) + kv * (D * KE) + at
+                                                       : reinterpret_cast<const char*>(geo.v_codes) + kv * (D * VE) + (at - Lds::k_bytes));
+            }
+            src_scale = uniform_ptr(scale_of_k ? reinterpret_cast<const char*>(geo.k_scales + kv * NB) + wave * kScalePiece
+                                               : reinterpret_cast<const char*>(geo.v_scales + kv * NB) + (wave * kScalePiece - Lds::scale_bytes));
+        };
+        auto fetch = [&]() __attribute__((always_inline)) {
+            if (run_left == 0) locate();
+            const uint32_t to = lds_offset(s_raw) + next % Lds::bufs * Lds::raw;
+#pragma unroll
+            for (uint32_t x = 0; x < kPieces; ++x) {
                 const uint32_t at = (wave + x * kChunkWaves) * 1024;
                 if (at < Lds::k_bytes + Lds::v_bytes)  // (12 KiB in the mixed modes at D = 128)
-                    copy_to_lds((at < Lds::k_bytes ? k + at : v + (at - Lds::k_bytes)) + lane * 16, to + at);
+                    copy_to_lds_from(src[x], lane * 16, to + at);
+                src[x] += at < Lds::k_bytes ? kChunk * D * KE : kChunk * D * VE;
             }
             if constexpr (!(KF16 && VF16)) {
-                constexpr uint32_t kEach = 2 * Lds::scale_bytes / kChunkWaves;  // of K's, then of V's
-                const uint32_t at = wave * kEach;
-                const bool of_k = at < Lds::scale_bytes;
-                if (lane < kEach / 16 && !(of_k ? KF16 : VF16))
-                    copy_to_lds(reinterpret_cast<const char*>(of_k ? geo.k_scales + kv * NB : geo.v_scales + kv * NB) +
-                                    (of_k ? at : at - Lds::scale_bytes) + lane * 16,
-                                to + Lds::k_bytes + Lds::v_bytes + at);
+                if (!(scale_of_k ? KF16 : VF16) && lane < kScalePiece / 16)
+                    copy_to_lds_from(src_scale, lane * 16, to + Lds::k_bytes + Lds::v_bytes + wave * kScalePiece);
+                src_scale += Lds::scale_bytes;
             }
+            ++next;
+            --run_left;
         };
         // Keys of the step that no row of the item sees may hold anything: their values are zeroed.
         auto unseen = [&](uint32_t t) __attribute__((always_inline)) {
             return (t >= span.past) | ((t < span.vis.lo) & (t >= a.sinks));
         };
-        // V's scales, two blocks of one key per thread, in the order of V's units.
-        auto order_scales = [&](uint32_t i) __attribute__((always_inline)) {
-            if (!VF16 && tid < 16 * NB) {
-                const uint32_t key = tid / (NB / 2), blk = tid % (NB / 2) * 2;
-                uint32_t w = *reinterpret_cast<const uint32_t*>(s_raw + i % Lds::bufs * Lds::raw + Lds::k_bytes + Lds::v_bytes +
-                                                                Lds::scale_bytes + tid * 4);
-                if (unseen(span.vis.step(i) * kChunk + key)) w = 0;
-                _Float16* to = s_vsc + (i & 1) * D + blk * 32 + ((key >> 2) & 3) * 8 + (key >> 4) * 4 + (key & 3);
-                to[0] = tile_scale(static_cast<uint16_t>(w & 0xffffu));
-                to[32] = tile_scale(static_cast<uint16_t>(w >> 16));
-            }
+        // Whether the step at tok0 holds such keys.
+        auto edge = [&](uint32_t tok0) __attribute__((always_inline)) {
+            return (tok0 + kChunk > span.past) | ((tok0 < span.vis.lo) & (tok0 + kChunk > a.sinks));
         };
-        // A step's codes to fp16: each thread 16 codes of K and / or of V.
+        // V's scales in the order of V's units: each of the first D / 2 threads puts those of two keys, one
+        // behind the other in a unit, together.
+        auto order_scales = [&](uint32_t i) __attribute__((always_inline)) {
+            if (VF16 || wave >= D / 128) return;
+            const uint32_t t = here(), blk = t / 16, x = t % 16 * 2;  // element x of the block's 32: G = x / 8, J = x / 4 % 2
+            const uint32_t key = x / 4 % 2 * 16 + x / 8 * 4 + x % 4;
+            const _Float16* from = reinterpret_cast<const _Float16*>(s_raw + i % Lds::bufs * Lds::raw + Lds::k_bytes + Lds::v_bytes + Lds::scale_bytes) +
+                                   key * NB + blk;
+            half2v w = {from[0], from[NB]};
+            const uint32_t tok0 = uniform(span.vis.step(i) * kChunk);
+            if (edge(tok0)) {
+                w[0] = unseen(tok0 + key) ? static_cast<_Float16>(0.0f) : w[0];
+                w[1] = unseen(tok0 + key + 1) ? static_cast<_Float16>(0.0f) : w[1];
+            }
+            *reinterpret_cast<half2v*>(s_vsc + (i & 1) * D + 2 * t) = tile_scales(w);
+        };
+        // A step's codes to fp16: each thread 16 codes of K and / or of V (D = 128: the first four
+        // waves K's, the others V's).
         constexpr bool kBoth = D == 256;
-        auto convert = [&](uint32_t i) __attribute__((always_inline)) {
-            const uint32_t idx = kBoth ? tid : tid & 255u;
+        auto convert_k = [&](uint32_t i) __attribute__((always_inline)) {
+            const uint32_t idx = here();
             const uint8_t* raw = s_raw + i % Lds::bufs * Lds::raw;
             half8* tile = s_tile + (i & 1) * Lds::units;
-            if (kBoth || tid < 256) {
+            if (kBoth || wave < 4) {
                 // key 16 T + m, dims 64 c + 8 g and 64 c + 32 + 8 g
                 const uint32_t T = idx / D, c = idx / 64 % (D / 64), g = idx / 16 % 4, m = idx % 16;
                 half8* to = tile + (8 * c + g) * kChunk + 16 * T + m;
@@ -424,12 +456,17 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
                     to[4 * kChunk] = __builtin_bit_cast(half8, from[1]);
                 } else {
                     const uint4 w = from[0];
-                    const uint32_t f = *reinterpret_cast<const uint32_t*>(raw + Lds::k_bytes + Lds::v_bytes + ((16 * T + m) * NB + 2 * c) * 2);
-                    to[0] = codes8_to_half8(w.x, w.y) * tile_scale(static_cast<uint16_t>(f & 0xffffu));
-                    to[4 * kChunk] = codes8_to_half8(w.z, w.w) * tile_scale(static_cast<uint16_t>(f >> 16));
+                    const half2v f = tile_scales(*reinterpret_cast<const half2v*>(raw + Lds::k_bytes + Lds::v_bytes + ((16 * T + m) * NB + 2 * c) * 2));
+                    to[0] = codes8_to_half8(w.x, w.y) * f[0];
+                    to[4 * kChunk] = codes8_to_half8(w.z, w.w) * f[1];
                 }
             }
-            if (kBoth || tid >= 256) {
+        };
+        auto convert_v = [&](uint32_t i) __attribute__((always_inline)) {
+            const uint32_t idx = kBoth ? here() : here() & 255u;
+            const uint8_t* raw = s_raw + i % Lds::bufs * Lds::raw;
+            half8* tile = s_tile + (i & 1) * Lds::units;
+            if (kBoth || wave >= 4) {
                 // dim d, keys of units 2x and 2x + 1
                 const uint32_t d = idx / 2, x = idx % 2;
                 half8* to = tile + Lds::k_units + 2 * x * Lds::v_row + d;
@@ -437,7 +474,7 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
                 if constexpr (VF16) {
                     half8 v[2] = {__builtin_bit_cast(half8, from[0]), __builtin_bit_cast(half8, from[VF16 ? 1 : 0])};
                     const uint32_t tok0 = uniform(span.vis.step(i) * kChunk);
-                    if (tok0 + kChunk > span.past || (tok0 < span.vis.lo && tok0 + kChunk > a.sinks)) {
+                    if (edge(tok0)) {
 #pragma unroll
                         for (uint32_t u = 0; u < 2; ++u)
 #pragma unroll
@@ -462,38 +499,44 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
 #pragma unroll
             for (uint32_t x = 0; x < 16; ++x) O[mt][x] = 0.0f;
 
-        if (s0 < s1) {
-            lds_barrier();  // the previous item's tiles and ring have been read
-            for (uint32_t i = s0; i < min(s0 + Lds::bufs, s1); ++i) fetch(i);
-            wait_vmem();
-            lds_barrier();
-            order_scales(s0);
-            if (s0 + 1 < s1) order_scales(s0 + 1);
-            lds_barrier();
-            convert(s0);
-        }
-        for (uint32_t s = s0; s < s1; ++s) {
-            // The step that is `landed` ahead is whole in the ring, of every wave's copies.
-            if (s != s0) {
-                if (KF16 == VF16 && s + Lds::bufs - 1 < s1) wait_vmem_le<(Lds::bufs - 1 - Lds::landed) * Lds::ops>();
-                else wait_vmem();
-            }
-            lds_barrier();
-            if (s + Lds::bufs < s1) fetch(s + Lds::bufs);  // where step s was, which is a tile now
-            if (s + 2 < s1) order_scales(s + 2);
-            if (s + 1 < s1) convert(s + 1);
-
+        // Whether this wave's rows see anything of a step (wave-uniform).
+        auto seen = [&](uint32_t s) __attribute__((always_inline)) {
             const uint32_t tok0 = uniform(span.vis.step(s) * kChunk);
-            // Nothing of the step is seen by this wave's rows (wave-uniform)?
-            if (!wave_live || tok0 >= past_z || (a.window != 0 && tok0 + kChunk <= low_a && tok0 >= a.sinks)) continue;
-            const bool whole = tok0 + kChunk <= past_a && (a.window == 0 || tok0 + kChunk <= a.sinks || tok0 >= low_z);
-            const half8* tile = s_tile + (s & 1) * Lds::units;
-            float16v S;
+            return wave_live & (tok0 < past_z) & ((a.window == 0) | (tok0 + kChunk > low_a) | (tok0 < a.sinks));
+        };
+        half8 qf[NQ];
+        float16v S;
+        half8 P[2];
+        // O^T += V^T P^T of step s - 1 (VALUES), then S^T = K Q^T of step s (SCORES): one run of MFMAs
+        // whose fragments are read kAhead ahead.
+        auto multiply = [&](auto with_values, auto with_scores, uint32_t s) __attribute__((always_inline)) {
+            constexpr uint32_t NV = decltype(with_values)::value ? 2 * NB : 0, N = NV + (decltype(with_scores)::value ? NQ : 0);
+            // value fragment c: dims 32 (c / 2) .., keys of units 2 (c % 2) + hh; key fragment: dims 16 c + 8 hh ..
+            const half8* v = s_tile + ((s - 1) & 1) * Lds::units + Lds::k_units + hh * Lds::v_row + n;
+            const half8* k = s_tile + (s & 1) * Lds::units + hh * kChunk + n;
+            auto at = [&](uint32_t c) __attribute__((always_inline)) {
+                return c < NV ? v[c / 2 * kChunk + c % 2 * 2 * Lds::v_row] : k[(c - NV) * 2 * kChunk];
+            };
+            half8 f[kAhead];
 #pragma unroll
-            for (uint32_t x = 0; x < 16; ++x) S[x] = 0.0f;
-            mfma_pairs<NQ>(tile + hh * kChunk + n, 2 * kChunk, [&](uint32_t k, half8 f) __attribute__((always_inline)) {
-                S = mfma_32x32x16(f, qf[k], S);
-            });
+            for (uint32_t c = 0; c < kAhead; ++c) f[c] = at(c);
+            if constexpr (decltype(with_scores)::value)
+#pragma unroll
+                for (uint32_t x = 0; x < 16; ++x) S[x] = 0.0f;
+            __builtin_amdgcn_sched_barrier(0);  // the scheduler would move reads to their use, or all of them up here
+#pragma unroll
+            for (uint32_t c = 0; c < N; ++c) {
+                if (c < NV) O[c / 2] = mfma_32x32x16(f[c % kAhead], P[c % 2], O[c / 2]);
+                else S = mfma_32x32x16(f[c % kAhead], qf[c - NV], S);
+                if (c + kAhead < N) f[c % kAhead] = at(c + kAhead);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        const std::true_type yes{};
+        const std::false_type no{};
+        auto softmax = [&](uint32_t s) __attribute__((always_inline)) {
+            const uint32_t tok0 = uniform(span.vis.step(s) * kChunk);
+            const bool whole = (tok0 + kChunk <= past_a) & ((a.window == 0) | (tok0 + kChunk <= a.sinks) | (tok0 >= low_z));
             if (!whole) {
 #pragma unroll
                 for (uint32_t x = 0; x < 16; ++x) {
@@ -501,9 +544,9 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
                     S[x] = (t >= past) | ((t < low) & (t >= a.sinks)) ? -INFINITY : S[x];
                 }
             }
-            float top = S[0];
-#pragma unroll
-            for (uint32_t x = 1; x < 16; ++x) top = fmaxf(top, S[x]);
+            // (fmaxf would first quieten each of its inputs)
+            float top = max3(max3(max3(S[0], S[1], S[2]), max3(S[3], S[4], S[5]), max3(S[6], S[7], S[8])),
+                             max3(S[9], S[10], S[11]), max3(S[12], S[13], max3(S[14], S[15], S[15])));
             top = swap32_reduce(top, MaxOp{}) * a.scale_log2;
             if (__any(top > m_run + kSlack)) {
                 const float to = fmaxf(m_run, top);
@@ -514,18 +557,113 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
                 for (uint32_t mt = 0; mt < NB; ++mt) O[mt] *= f;
             }
             const float use = m_run == -INFINITY ? 0.0f : m_run;
-            half8 P[2];
 #pragma unroll
-            for (uint32_t x = 0; x < 16; ++x) {
-                const float p = exp2_fast(fmaf(S[x], a.scale_log2, -use));
-                l_run += p;
-                P[x / 4 % 2][x % 4 + x / 8 * 4] = static_cast<_Float16>(p);
+            for (uint32_t x = 0; x < 16; ++x)
+                P[x / 4 % 2][x % 4 + x / 8 * 4] = static_cast<_Float16>(exp2_fast(fmaf(S[x], a.scale_log2, -use)));
+            // the sum of the probabilities as the second product takes them
+            const half2v one = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
+            float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (uint32_t x = 0; x < 8; x += 2)
+#pragma unroll
+                for (uint32_t u = 0; u < 2; ++u) sum[u] = __builtin_amdgcn_fdot2(half2v{P[u][x], P[u][x + 1]}, one, sum[u], false);
+            l_run += sum[0] + sum[1];
+        };
+        if (s0 < s1) {
+            lds_barrier();  // the previous item's tiles and ring have been read
+            for (uint32_t i = s0; i < min(s0 + Lds::bufs, s1); ++i) fetch();
+        }
+        with_type(a.q_dtype, [&](auto t) __attribute__((always_inline)) {
+#pragma unroll
+            for (uint32_t k = 0; k < NQ; ++k) qf[k] = load_query<decltype(t)>(a.q, row_at + 16 * k + 8 * hh);
+        });
+        if (a.negate)
+#pragma unroll
+            for (uint32_t k = 0; k < NQ; ++k) qf[k] = -qf[k];
+        // The query has arrived: otherwise its loads are waited for in every step, and with them
+        // the copies, which the compiler does not count.
+#pragma unroll
+        for (uint32_t k = 0; k < NQ; ++k) asm volatile("" : "+v"(qf[k]));
+
+        if (s0 < s1) {
+            wait_vmem();
+            lds_barrier();
+            order_scales(s0);
+            if (!Lds::turns && s0 + 1 < s1) order_scales(s0 + 1);
+            lds_barrier();
+            convert_k(s0);
+            if (!Lds::turns || wave >= 4) convert_v(s0);
+        }
+        if constexpr (Lds::turns) {
+            // The two waves of a SIMD take turns: while waves 0..3 multiply (values of step s - 1, scores
+            // of step s), waves 4..7 do what is left to the vector unit (softmax of step s - 1, codes to
+            // fp16), and the other way round.  With t = s - s0, in interval 2t the first half multiplies,
+            // in 2t + 1 it computes; the second half is one interval later.  A tile's K is
+            // whole before interval 2t: its codes are converted by the first half in 2t - 1, by the
+            // second in 2t - 2; its V before 2t + 2: in 2t + 1 and 2t.  Each overwrites what was
+            // last read an interval before or earlier: K of step s - 2 in 2t - 3, V of step s - 2 in
+            // 2t - 1.  The ring's place of step s is free from 2t + 2.
+            // A wave without rows only copies and converts.  (What a wave's rows do not see of the item's
+            // steps is multiplied and masked: with a branch around it the accumulators would be held
+            // twice.)
+            const bool second = wave >= 4;
+            auto steps_of = [&](auto live) __attribute__((always_inline)) {
+                constexpr bool kLive = decltype(live)::value;
+                if (second) {
+                    if (s0 + 1 < s1) convert_k(s0 + 1);
+                    lds_barrier();
+                }
+                lds_barrier();
+                if constexpr (kLive) multiply(no, yes, s0);
+                // (The last pass multiplies scores that nothing uses, of whatever the tile holds: leaving
+                // the loop in front of them would hold the accumulators twice.)
+                for (uint32_t s = s0; s < s1; ++s) {
+                    if (second) wait_vmem();  // step s + 2 has landed
+                    lds_barrier();
+                    if (s != s0 && s + 3 < s1) fetch();  // step s + 3
+                    if (!second && s + 1 < s1) order_scales(s + 1);
+                    if constexpr (kLive) softmax(s);
+                    if (second) {
+                        if (s + 2 < s1) convert_k(s + 2);
+                        if (s + 1 < s1) convert_v(s + 1);
+                    } else {
+                        if (s + 1 < s1) convert_k(s + 1);
+                        convert_v(s);
+                        if (s + 3 < s1) wait_vmem_le<Lds::ops>();  // step s + 2 has landed
+                        else wait_vmem();
+                    }
+                    lds_barrier();
+                    if constexpr (kLive) {
+                        __builtin_amdgcn_s_setprio(1);
+                        multiply(yes, yes, s + 1);
+                        __builtin_amdgcn_s_setprio(0);
+                    }
+                }
+                if (!second) lds_barrier();
+            };
+            if (s0 < s1) {
+                if (wave_live) steps_of(yes);
+                else steps_of(no);
             }
-#pragma unroll
-            for (uint32_t u = 0; u < 2; ++u)
-                mfma_pairs<NB>(tile + Lds::k_units + (2 * u + hh) * Lds::v_row + n, kChunk, [&](uint32_t mt, half8 f) __attribute__((always_inline)) {
-                    O[mt] = mfma_32x32x16(f, P[u], O[mt]);
-                });
+        } else {
+            for (uint32_t s = s0; s < s1; ++s) {
+                // The step that is `landed` ahead is whole in the ring, of every wave's copies.
+                if (s != s0) {
+                    if (KF16 == VF16 && s + Lds::bufs - 1 < s1) wait_vmem_le<(Lds::bufs - 1 - Lds::landed) * Lds::ops>();
+                    else wait_vmem();
+                }
+                lds_barrier();
+                if (s + Lds::bufs < s1) fetch();  // where step s was, which is a tile now
+                if (s + 2 < s1) order_scales(s + 2);
+                if (s + 1 < s1) {
+                    convert_k(s + 1);
+                    convert_v(s + 1);
+                }
+                if (!seen(s)) continue;
+                multiply(no, yes, s);
+                softmax(s);
+                multiply(yes, no, s + 1);
+            }
         }
         l_run = swap32_reduce(l_run, AddOp{});
         const float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;  // a token that sees no key: zeros
@@ -711,6 +849,10 @@ extern "C" miikv_status miikv_chunk_attn(const miikv_view* view, const void* q, 
     a.out_dtype = out_dtype;
     a.most_items = static_cast<uint32_t>(p.items);
     a.parts = p.parts;
+    a.page_steps = view->page_tokens / kChunk;
+    // mulhi(x, ceil(2^32 / d)) == x / d where x * d < 2^32
+    const uint64_t steps = (static_cast<uint64_t>(max_context) + kChunk - 1) / kChunk;
+    a.page_magic = steps * a.page_steps < 0xffffffffu ? static_cast<uint32_t>((0x100000000ull + a.page_steps - 1) / a.page_steps) : 0u;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     a.head = reinterpret_cast<uint32_t*>(ws);
     a.items = reinterpret_cast<ChunkItem*>(ws + 256);
