@@ -37,6 +37,8 @@ constexpr uint32_t kRows = 32 * kChunkWaves;  // rows of an item
 constexpr uint32_t kItemCost = 4;             // an item's fixed cost, in steps
 constexpr uint32_t kMinUnits = 12;            // units per workgroup, at least
 constexpr uint32_t kMaxParts = 256;           // one workgroup per CU
+constexpr uint32_t kTileItems = 2;            // items per (sequence, kv head) from which on keys are expanded first
+constexpr uint64_t kMaxTileBytes = 1ull << 30;
 constexpr float kSlack = 8.0f;                // the maximum may grow by this (log2) before sums are rescaled
 
 struct ChunkItem {
@@ -71,6 +73,8 @@ struct ChunkArgs {
     // workspace
     uint32_t* head;      // [0] items of one kv head, [1] units of one kv head, [2] units per part
     ChunkItem* items;    // [most_items]
+    uint32_t most_steps; // tiles of a (sequence, kv head)
+    const half8* tiles;  // [batch][kv_heads][most_steps]
     _Float16* rec_o;     // [2 * parts][kRows][D]: outputs over the part's keys
     float2* rec_ml;      // [2 * parts][kRows]: maximum (log2 units) and sum
 };
@@ -228,17 +232,123 @@ struct ChunkLds {
     static constexpr uint32_t bytes = 2 * units * 16 + bufs * raw + vsc_bytes;
 };
 
+// With tiles that expand_kernel has made: a ring of them, K units [D / 8][32 keys] and V units
+// [4][D] of 8 values.
+template <uint32_t D>
+struct TileLds {
+    static constexpr uint32_t k_units = D / 8 * kChunk;
+    static constexpr uint32_t v_row = D;
+    static constexpr uint32_t units = k_units + 4 * v_row;
+    static constexpr uint32_t bufs = D == 128 ? 8 : 4;
+    static constexpr uint32_t ops = units * 16 / 1024 / kChunkWaves;
+    static constexpr uint32_t bytes = bufs * units * 16;
+};
+
+// Tile of a step (counted among the steps that any token of the chunk sees, `all`) of (b, h).
+__device__ __forceinline__ const half8* tile_at(const ChunkArgs& a, uint32_t b, uint32_t h, const Visible& all, uint32_t step, uint32_t units) {
+    const uint32_t i = step < all.head ? step : all.head + (step - all.first);
+    return a.tiles + ((static_cast<size_t>(b) * a.g.kv_heads + h) * a.most_steps + i) * units;
+}
+
+// One step of (sequence z, kv head y) as an fp16 tile: code * scale, rounded once.  Keys that no
+// token of the chunk sees may hold anything: their values become 0.
+// Bound: HBM (the codes once, the tiles once).
 template <uint32_t D, bool KF16, bool VF16>
+__global__ void __launch_bounds__(256) expand_kernel(ChunkArgs a) {
+    constexpr uint32_t NB = D / 32, KE = KF16 ? 2 : 1, VE = VF16 ? 2 : 1, kRuns = 2 * D;  // 16 codes each, of K and of V
+    using Lds = TileLds<D>;
+    const uint32_t b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
+    const Geo& geo = a.g;
+    const Chunk c = chunk_of_uniform(a, b);
+    if (c.tokens == 0) return;
+    const Visible all = visible_steps(c.length, c.tokens, a.window, a.sinks);
+    if (blockIdx.x >= all.steps()) return;
+    const uint32_t tok0 = all.step(blockIdx.x) * kChunk;
+    uint32_t page = 0, tp = tok0;
+    if (geo.layout == MIIKV_LAYOUT_PAGED) {
+        const uint32_t e = tok0 / geo.page_tokens;
+        tp = tok0 - e * geo.page_tokens;
+        page = min(static_cast<uint32_t>(scalar_load(geo.table + static_cast<size_t>(b) * geo.table_stride + e)), geo.num_pages - 1);
+    }
+    const size_t row = (static_cast<size_t>(page) * geo.kv_heads + h) * geo.page_tokens + tp;
+    half8* tile = const_cast<half8*>(tile_at(a, b, h, all, tok0 / kChunk, Lds::units));
+    const uint4* kc = reinterpret_cast<const uint4*>(geo.k_codes + row * (D * KE));
+    const uint4* vc = reinterpret_cast<const uint4*>(geo.v_codes + row * (D * VE));
+    uint4 kw[kRuns / 256][KE], vw[kRuns / 256][VE];
+    half2v ks[kRuns / 256];
+#pragma unroll
+    for (uint32_t j = 0; j < kRuns / 256; ++j) {
+        const uint32_t idx = j * 256 + tid;
+#pragma unroll
+        for (uint32_t e = 0; e < KE; ++e) kw[j][e] = kc[idx * KE + e];
+#pragma unroll
+        for (uint32_t e = 0; e < VE; ++e) vw[j][e] = vc[idx * VE + e];
+        if constexpr (!KF16)
+            ks[j] = *reinterpret_cast<const half2v*>(geo.k_scales + (row + 16 * (idx / D) + idx % 16) * NB + 2 * (idx / 64 % (D / 64)));
+    }
+    auto unseen = [&](uint32_t t) { return (t >= c.length) | ((t < all.lo) & (t >= a.sinks)); };
+    __shared__ __align__(16) _Float16 s_vsc[D];  // V's scales in the order of its units
+    if (!VF16 && tid < D / 2) {
+        const uint32_t key = tid / (NB / 2), blk = tid % (NB / 2) * 2;
+        half2v w = tile_scales(*reinterpret_cast<const half2v*>(geo.v_scales + row * NB + 2 * tid));
+        if (unseen(tok0 + key)) w = half2v{static_cast<_Float16>(0.0f), static_cast<_Float16>(0.0f)};
+        _Float16* to = s_vsc + blk * 32 + (key / 4 % 4) * 8 + key / 16 * 4 + key % 4;
+        to[0] = w[0];
+        to[32] = w[1];
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t j = 0; j < kRuns / 256; ++j) {
+        const uint32_t idx = j * 256 + tid;
+        {  // key 16 T + m, dims 64 c + 8 g and 64 c + 32 + 8 g
+            half8* to = tile + (8 * (idx / 64 % (D / 64)) + idx / 16 % 4) * kChunk + 16 * (idx / D) + idx % 16;
+            if constexpr (KF16) {
+                to[0] = __builtin_bit_cast(half8, kw[j][0]);
+                to[4 * kChunk] = __builtin_bit_cast(half8, kw[j][KE - 1]);
+            } else {
+                const half2v f = tile_scales(ks[j]);
+                to[0] = codes8_to_half8(kw[j][0].x, kw[j][0].y) * f[0];
+                to[4 * kChunk] = codes8_to_half8(kw[j][0].z, kw[j][0].w) * f[1];
+            }
+        }
+        {  // dim d, keys of units 2x and 2x + 1
+            const uint32_t d = idx / 2, x = idx % 2;
+            half8* to = tile + Lds::k_units + 2 * x * Lds::v_row + d;
+            half8 v[2];
+            if constexpr (VF16) {
+                v[0] = __builtin_bit_cast(half8, vw[j][0]);
+                v[1] = __builtin_bit_cast(half8, vw[j][VE - 1]);
+#pragma unroll
+                for (uint32_t u = 0; u < 2; ++u)
+#pragma unroll
+                    for (uint32_t y = 0; y < 8; ++y)
+                        v[u][y] = unseen(tok0 + 16 * (y / 4) + 4 * (2 * x + u) + y % 4) ? static_cast<_Float16>(0.0f) : v[u][y];
+            } else {
+                const half8* f = reinterpret_cast<const half8*>(s_vsc + d / 32 * 32 + 16 * x);
+                v[0] = codes8_to_half8(vw[j][0].x, vw[j][0].y) * f[0];
+                v[1] = codes8_to_half8(vw[j][0].z, vw[j][0].w) * f[1];
+            }
+            to[0] = v[0];
+            to[Lds::v_row] = v[1];
+        }
+    }
+}
+
+// TILES: steps come as tiles that expand_kernel has made (KF16 and VF16 are of no account), else
+// as the cache holds them.
+template <uint32_t D, bool KF16, bool VF16, bool TILES>
 __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per_eu(2))) chunk_kernel(ChunkArgs a) {
     constexpr uint32_t NB = D / 32;
     constexpr uint32_t NQ = D / 16;  // K-axis chunks of the first product
     constexpr uint32_t KE = KF16 ? 2 : 1, VE = VF16 ? 2 : 1;
     constexpr uint32_t kAhead = D == 128 ? 8 : 4;  // fragments read ahead of their MFMAs
-    using Lds = ChunkLds<D, KF16, VF16>;
+    using Raw = ChunkLds<D, KF16, VF16>;
+    using Lds = typename std::conditional<TILES, TileLds<D>, Raw>::type;
     extern __shared__ __align__(16) uint8_t lds[];
-    half8* const s_tile = reinterpret_cast<half8*>(lds);  // two tiles
-    uint8_t* const s_raw = lds + 2 * Lds::units * 16;
-    _Float16* const s_vsc = reinterpret_cast<_Float16*>(s_raw + Lds::bufs * Lds::raw);  // [2][NB][4][8]
+    constexpr uint32_t kTiles = TILES ? Lds::bufs : 2;
+    half8* const s_tile = reinterpret_cast<half8*>(lds);  // [kTiles]
+    uint8_t* const s_raw = lds + 2 * Raw::units * 16;
+    _Float16* const s_vsc = reinterpret_cast<_Float16*>(s_raw + Raw::bufs * Raw::raw);  // [2][NB][4][8]
     uint32_t* const s_first = reinterpret_cast<uint32_t*>(lds + Lds::bytes);  // [batch + 1]: items before sequence b
     uint32_t* const s_start = s_first + a.batch + 1;                          // [most_items + 1]: units before item i
     __shared__ uint32_t s_wave[kChunkWaves];
@@ -362,15 +472,21 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
         // the KiB of codes, and each copies an eighth of the scales.  A wave keeps the addresses of
         // its pieces and steps them on; at a page's end (and where the steps of the first tokens end) they
         // are made anew, from 64 entries of the block table held by the lanes.
-        constexpr uint32_t kPieces = (Lds::k_bytes + Lds::v_bytes + 1024 * kChunkWaves - 1) / 1024 / kChunkWaves;
-        constexpr uint32_t kScalePiece = 2 * Lds::scale_bytes / kChunkWaves;  // of K's, then of V's
+        constexpr uint32_t kPieces = TILES ? 1 : (Raw::k_bytes + Raw::v_bytes + 1024 * kChunkWaves - 1) / 1024 / kChunkWaves;
+        constexpr uint32_t kScalePiece = 2 * Raw::scale_bytes / kChunkWaves;  // of K's, then of V's
         const bool scale_of_k = wave < kChunkWaves / 2;
         const char* src[kPieces];
         const char* src_scale = nullptr;
         uint32_t next = s0, run_left = 0;
         uint32_t tab = 0, tab0 = 0x80000000u;  // (none yet)
+        const Visible all = visible_steps(c.length, c.tokens, a.window, a.sinks);  // what any token of the chunk sees
         auto locate = [&]() __attribute__((always_inline)) {
             const uint32_t st = uniform(span.vis.step(next));
+            if constexpr (TILES) {
+                run_left = next < span.vis.head ? span.vis.head - next : 0x7fffffffu;
+                src[0] = uniform_ptr(reinterpret_cast<const char*>(tile_at(a, b, h, all, st, Lds::units)) + wave * 1024);
+                return;
+            }
             uint32_t page = 0, slot = st;
             run_left = 0x7fffffffu;
             if (geo.layout == MIIKV_LAYOUT_PAGED) {
@@ -391,26 +507,36 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
 #pragma unroll
             for (uint32_t x = 0; x < kPieces; ++x) {
                 const uint32_t at = (wave + x * kChunkWaves) * 1024;
-                src[x] = uniform_ptr(at < Lds::k_bytes ? reinterpret_cast<const char*>(geo.k_codes) + kv * (D * KE) + at
-                                                       : reinterpret_cast<const char*>(geo.v_codes) + kv * (D * VE) + (at - Lds::k_bytes));
+                src[x] = uniform_ptr(at < Raw::k_bytes ? reinterpret_cast<const char*>(geo.k_codes) + kv * (D * KE) + at
+                                                       : reinterpret_cast<const char*>(geo.v_codes) + kv * (D * VE) + (at - Raw::k_bytes));
             }
             src_scale = uniform_ptr(scale_of_k ? reinterpret_cast<const char*>(geo.k_scales + kv * NB) + wave * kScalePiece
-                                               : reinterpret_cast<const char*>(geo.v_scales + kv * NB) + (wave * kScalePiece - Lds::scale_bytes));
+                                               : reinterpret_cast<const char*>(geo.v_scales + kv * NB) + (wave * kScalePiece - Raw::scale_bytes));
         };
         auto fetch = [&]() __attribute__((always_inline)) {
             if (run_left == 0) locate();
-            const uint32_t to = lds_offset(s_raw) + next % Lds::bufs * Lds::raw;
+            if constexpr (TILES) {
+                const uint32_t to = lds_offset(s_tile) + next % Lds::bufs * Lds::units * 16 + wave * 1024;
+#pragma unroll
+                for (uint32_t x = 0; x < TileLds<D>::ops; ++x)
+                    copy_to_lds_from(src[0] + x * kChunkWaves * 1024, lane * 16, to + x * kChunkWaves * 1024);
+                src[0] += Lds::units * 16;
+                ++next;
+                --run_left;
+                return;
+            }
+            const uint32_t to = lds_offset(s_raw) + next % Raw::bufs * Raw::raw;
 #pragma unroll
             for (uint32_t x = 0; x < kPieces; ++x) {
                 const uint32_t at = (wave + x * kChunkWaves) * 1024;
-                if (at < Lds::k_bytes + Lds::v_bytes)  // (12 KiB in the mixed modes at D = 128)
+                if (at < Raw::k_bytes + Raw::v_bytes)  // (12 KiB in the mixed modes at D = 128)
                     copy_to_lds_from(src[x], lane * 16, to + at);
-                src[x] += at < Lds::k_bytes ? kChunk * D * KE : kChunk * D * VE;
+                src[x] += at < Raw::k_bytes ? kChunk * D * KE : kChunk * D * VE;
             }
             if constexpr (!(KF16 && VF16)) {
                 if (!(scale_of_k ? KF16 : VF16) && lane < kScalePiece / 16)
-                    copy_to_lds_from(src_scale, lane * 16, to + Lds::k_bytes + Lds::v_bytes + wave * kScalePiece);
-                src_scale += Lds::scale_bytes;
+                    copy_to_lds_from(src_scale, lane * 16, to + Raw::k_bytes + Raw::v_bytes + wave * kScalePiece);
+                src_scale += Raw::scale_bytes;
             }
             ++next;
             --run_left;
@@ -429,7 +555,7 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
             if (VF16 || wave >= D / 128) return;
             const uint32_t t = here(), blk = t / 16, x = t % 16 * 2;  // element x of the block's 32: G = x / 8, J = x / 4 % 2
             const uint32_t key = x / 4 % 2 * 16 + x / 8 * 4 + x % 4;
-            const _Float16* from = reinterpret_cast<const _Float16*>(s_raw + i % Lds::bufs * Lds::raw + Lds::k_bytes + Lds::v_bytes + Lds::scale_bytes) +
+            const _Float16* from = reinterpret_cast<const _Float16*>(s_raw + i % Raw::bufs * Raw::raw + Raw::k_bytes + Raw::v_bytes + Raw::scale_bytes) +
                                    key * NB + blk;
             half2v w = {from[0], from[NB]};
             const uint32_t tok0 = uniform(span.vis.step(i) * kChunk);
@@ -444,8 +570,8 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
         constexpr bool kBoth = D == 256;
         auto convert_k = [&](uint32_t i) __attribute__((always_inline)) {
             const uint32_t idx = here();
-            const uint8_t* raw = s_raw + i % Lds::bufs * Lds::raw;
-            half8* tile = s_tile + (i & 1) * Lds::units;
+            const uint8_t* raw = s_raw + i % Raw::bufs * Raw::raw;
+            half8* tile = s_tile + (i & 1) * Raw::units;
             if (kBoth || wave < 4) {
                 // key 16 T + m, dims 64 c + 8 g and 64 c + 32 + 8 g
                 const uint32_t T = idx / D, c = idx / 64 % (D / 64), g = idx / 16 % 4, m = idx % 16;
@@ -456,7 +582,7 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
                     to[4 * kChunk] = __builtin_bit_cast(half8, from[1]);
                 } else {
                     const uint4 w = from[0];
-                    const half2v f = tile_scales(*reinterpret_cast<const half2v*>(raw + Lds::k_bytes + Lds::v_bytes + ((16 * T + m) * NB + 2 * c) * 2));
+                    const half2v f = tile_scales(*reinterpret_cast<const half2v*>(raw + Raw::k_bytes + Raw::v_bytes + ((16 * T + m) * NB + 2 * c) * 2));
                     to[0] = codes8_to_half8(w.x, w.y) * f[0];
                     to[4 * kChunk] = codes8_to_half8(w.z, w.w) * f[1];
                 }
@@ -464,13 +590,13 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
         };
         auto convert_v = [&](uint32_t i) __attribute__((always_inline)) {
             const uint32_t idx = kBoth ? here() : here() & 255u;
-            const uint8_t* raw = s_raw + i % Lds::bufs * Lds::raw;
-            half8* tile = s_tile + (i & 1) * Lds::units;
+            const uint8_t* raw = s_raw + i % Raw::bufs * Raw::raw;
+            half8* tile = s_tile + (i & 1) * Raw::units;
             if (kBoth || wave >= 4) {
                 // dim d, keys of units 2x and 2x + 1
                 const uint32_t d = idx / 2, x = idx % 2;
-                half8* to = tile + Lds::k_units + 2 * x * Lds::v_row + d;
-                const uint4* from = reinterpret_cast<const uint4*>(raw + Lds::k_bytes) + idx * VE;
+                half8* to = tile + Raw::k_units + 2 * x * Raw::v_row + d;
+                const uint4* from = reinterpret_cast<const uint4*>(raw + Raw::k_bytes) + idx * VE;
                 if constexpr (VF16) {
                     half8 v[2] = {__builtin_bit_cast(half8, from[0]), __builtin_bit_cast(half8, from[VF16 ? 1 : 0])};
                     const uint32_t tok0 = uniform(span.vis.step(i) * kChunk);
@@ -482,12 +608,12 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
                                 v[u][y] = unseen(tok0 + 16 * (y / 4) + 4 * (2 * x + u) + y % 4) ? static_cast<_Float16>(0.0f) : v[u][y];
                     }
                     to[0] = v[0];
-                    to[Lds::v_row] = v[1];
+                    to[Raw::v_row] = v[1];
                 } else {
                     const uint4 w = from[0];
                     const half8* f = reinterpret_cast<const half8*>(s_vsc + (i & 1) * D + d / 32 * 32 + 16 * x);
                     to[0] = codes8_to_half8(w.x, w.y) * f[0];
-                    to[Lds::v_row] = codes8_to_half8(w.z, w.w) * f[1];
+                    to[Raw::v_row] = codes8_to_half8(w.z, w.w) * f[1];
                 }
             }
         };
@@ -512,8 +638,8 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
         auto multiply = [&](auto with_values, auto with_scores, uint32_t s) __attribute__((always_inline)) {
             constexpr uint32_t NV = decltype(with_values)::value ? 2 * NB : 0, N = NV + (decltype(with_scores)::value ? NQ : 0);
             // value fragment c: dims 32 (c / 2) .., keys of units 2 (c % 2) + hh; key fragment: dims 16 c + 8 hh ..
-            const half8* v = s_tile + ((s - 1) & 1) * Lds::units + Lds::k_units + hh * Lds::v_row + n;
-            const half8* k = s_tile + (s & 1) * Lds::units + hh * kChunk + n;
+            const half8* v = s_tile + (s - 1) % kTiles * Lds::units + Lds::k_units + hh * Lds::v_row + n;
+            const half8* k = s_tile + s % kTiles * Lds::units + hh * kChunk + n;
             auto at = [&](uint32_t c) __attribute__((always_inline)) {
                 return c < NV ? v[c / 2 * kChunk + c % 2 * 2 * Lds::v_row] : k[(c - NV) * 2 * kChunk];
             };
@@ -571,7 +697,8 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
         };
         if (s0 < s1) {
             lds_barrier();  // the previous item's tiles and ring have been read
-            for (uint32_t i = s0; i < min(s0 + Lds::bufs, s1); ++i) fetch();
+            // (the query is waited for behind these: of tiles, no more than the first two steps)
+            for (uint32_t i = s0; i < min(s0 + (TILES ? 2 : Lds::bufs), s1); ++i) fetch();
         }
         with_type(a.q_dtype, [&](auto t) __attribute__((always_inline)) {
 #pragma unroll
@@ -588,13 +715,57 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
         if (s0 < s1) {
             wait_vmem();
             lds_barrier();
-            order_scales(s0);
-            if (!Lds::turns && s0 + 1 < s1) order_scales(s0 + 1);
-            lds_barrier();
-            convert_k(s0);
-            if (!Lds::turns || wave >= 4) convert_v(s0);
+            if constexpr (TILES) {
+                for (uint32_t i = s0 + 2; i < min(s0 + Lds::bufs, s1); ++i) fetch();
+            } else {
+                order_scales(s0);
+                if (!Raw::turns && s0 + 1 < s1) order_scales(s0 + 1);
+                lds_barrier();
+                convert_k(s0);
+                if (!Raw::turns || wave >= 4) convert_v(s0);
+            }
         }
-        if constexpr (Lds::turns) {
+        if constexpr (TILES) {
+            // The two waves of a SIMD take turns: while waves 0..3 multiply (values of step s - 1, scores of
+            // step s), waves 4..7 do the softmax of step s - 1, and the other way round.  With
+            // t = s - s0, the first half multiplies in interval 2t and computes in 2t + 1, the second half
+            // one interval later.  Step s is read from 2t to 2t + 3 and must have landed before 2t; its
+            // place is fetched into anew from 2t + 4 on, in the turns of step s + 2.
+            const bool second = wave >= 4;
+            auto steps_of = [&](auto live) __attribute__((always_inline)) {
+                constexpr bool kLive = decltype(live)::value;
+                if (second) lds_barrier();
+                if constexpr (kLive) multiply(no, yes, s0);
+                // (The last pass multiplies scores that nothing uses: leaving the loop in front of them would
+                // hold the accumulators twice.)
+                for (uint32_t s = s0; s < s1; ++s) {
+                    if (second) {  // step s + 1 has landed
+                        if (s + Lds::bufs - 3 < s1) wait_vmem_le<(Lds::bufs - 4) * TileLds<D>::ops>();
+                        else wait_vmem();
+                    }
+                    lds_barrier();
+                    if (s >= s0 + 2 && s + Lds::bufs - 2 < s1) fetch();  // step s + bufs - 2
+                    if constexpr (kLive) softmax(s);
+                    if (!second) {
+                        if (s + Lds::bufs - 2 < s1) wait_vmem_le<(Lds::bufs - 3) * TileLds<D>::ops>();
+                        else wait_vmem();
+                    }
+                    // (the exponentials would move behind the barrier, into the turn that multiplies)
+                    __builtin_amdgcn_sched_barrier(0);
+                    lds_barrier();
+                    if constexpr (kLive) {
+                        __builtin_amdgcn_s_setprio(1);
+                        multiply(yes, yes, s + 1);
+                        __builtin_amdgcn_s_setprio(0);
+                    }
+                }
+                if (!second) lds_barrier();
+            };
+            if (s0 < s1) {
+                if (wave_live) steps_of(yes);
+                else steps_of(no);
+            }
+        } else if constexpr (Raw::turns) {
             // The two waves of a SIMD take turns: while waves 0..3 multiply (values of step s - 1, scores
             // of step s), waves 4..7 do what is left to the vector unit (softmax of step s - 1, codes to
             // fp16), and the other way round.  With t = s - s0, in interval 2t the first half multiplies,
@@ -629,7 +800,7 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
                     } else {
                         if (s + 1 < s1) convert_k(s + 1);
                         convert_v(s);
-                        if (s + 3 < s1) wait_vmem_le<Lds::ops>();  // step s + 2 has landed
+                        if (s + 3 < s1) wait_vmem_le<Raw::ops>();  // step s + 2 has landed
                         else wait_vmem();
                     }
                     lds_barrier();
@@ -649,11 +820,11 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
             for (uint32_t s = s0; s < s1; ++s) {
                 // The step that is `landed` ahead is whole in the ring, of every wave's copies.
                 if (s != s0) {
-                    if (KF16 == VF16 && s + Lds::bufs - 1 < s1) wait_vmem_le<(Lds::bufs - 1 - Lds::landed) * Lds::ops>();
+                    if (KF16 == VF16 && s + Raw::bufs - 1 < s1) wait_vmem_le<(Raw::bufs - 1 - Raw::landed) * Raw::ops>();
                     else wait_vmem();
                 }
                 lds_barrier();
-                if (s + Lds::bufs < s1) fetch();  // where step s was, which is a tile now
+                if (s + Raw::bufs < s1) fetch();  // where step s was, which is a tile now
                 if (s + 2 < s1) order_scales(s + 2);
                 if (s + 1 < s1) {
                     convert_k(s + 1);
@@ -754,8 +925,10 @@ struct ChunkPlan {
     uint64_t items;  // of one kv head, at most
     uint32_t parts;
     size_t lds;
-    uint64_t item_bytes, o_bytes, ml_bytes;
-    uint64_t bytes() const { return 256 + item_bytes + o_bytes + ml_bytes; }
+    uint32_t steps;  // of a (sequence, kv head), at most
+    bool tiles;      // expand first
+    uint64_t item_bytes, o_bytes, ml_bytes, tile_bytes;
+    uint64_t bytes() const { return 256 + item_bytes + o_bytes + ml_bytes + tile_bytes; }
 };
 
 // Sizes and the plan's bounds; a status.
@@ -771,13 +944,17 @@ int chunk_plan(const miikv_view* v, uint32_t q_heads, uint32_t batch, uint32_t t
     if (rows > 0x7fffffffu || batch > 65535u || v->kv_heads > 65535u) return MIIKV_EUNSUPPORTED;
     // every sequence's last item may be a part of one
     p.items = std::min<uint64_t>(rows / kRows + batch, rows);
-    const uint64_t most = kItemCost + most_visible_steps(max_context, max_tokens, window, sinks);
+    p.steps = most_visible_steps(max_context, max_tokens, window, sinks);
+    const uint64_t most = kItemCost + p.steps;
     const uint64_t axis = p.items * most * v->kv_heads;
     if (axis / v->kv_heads / most != p.items || axis > 0xf0000000u) return MIIKV_EUNSUPPORTED;  // 32-bit places on the axis
     p.parts = static_cast<uint32_t>(std::min<uint64_t>(kMaxParts, (axis + kMinUnits - 1) / kMinUnits));
     const uint32_t D = v->head_dim;
-    p.lds = chunk_lds_bytes(D, mode_k_f16(v->quant_mode), mode_v_f16(v->quant_mode)) +
-            (static_cast<size_t>(batch) + 1 + p.items + 1) * sizeof(uint32_t);
+    const uint64_t tile_bytes = static_cast<uint64_t>(batch) * v->kv_heads * p.steps * (128u * D);
+    p.tiles = rows >= static_cast<uint64_t>(kTileItems) * kRows * batch && tile_bytes <= kMaxTileBytes && batch <= 65535u;
+    p.tile_bytes = p.tiles ? tile_bytes : 0u;
+    p.lds = p.tiles ? (D == 128 ? TileLds<128>::bytes : TileLds<256>::bytes) : chunk_lds_bytes(D, mode_k_f16(v->quant_mode), mode_v_f16(v->quant_mode));
+    p.lds += (static_cast<size_t>(batch) + 1 + p.items + 1) * sizeof(uint32_t);
     if (p.lds > 159 * 1024) return MIIKV_EUNSUPPORTED;
     p.item_bytes = up256(p.items * sizeof(ChunkItem));
     p.o_bytes = up256(2ull * p.parts * kRows * D * sizeof(uint16_t));
@@ -789,7 +966,13 @@ template <uint32_t D>
 int launch_chunk(const ChunkArgs& a, const ChunkPlan& p, bool kf, bool vf, hipStream_t s) {
     const dim3 grid((p.parts + 7) / 8 * 8);
     const auto go = [&](auto k, auto v) {
-        hipLaunchKernelGGL((chunk_kernel<D, decltype(k)::value, decltype(v)::value>), grid, dim3(kChunkThreads), p.lds, s, a);
+        constexpr bool KF = decltype(k)::value, VF = decltype(v)::value;
+        if (p.tiles) {
+            hipLaunchKernelGGL((expand_kernel<D, KF, VF>), dim3(p.steps, a.g.kv_heads, a.batch), dim3(256), 0, s, a);
+            hipLaunchKernelGGL((chunk_kernel<D, false, false, true>), grid, dim3(kChunkThreads), p.lds, s, a);
+        } else {
+            hipLaunchKernelGGL((chunk_kernel<D, KF, VF, false>), grid, dim3(kChunkThreads), p.lds, s, a);
+        }
     };
     const auto with_v = [&](auto k) { vf ? go(k, std::true_type{}) : go(k, std::false_type{}); };
     kf ? with_v(std::true_type{}) : with_v(std::false_type{});
@@ -858,6 +1041,8 @@ extern "C" miikv_status miikv_chunk_attn(const miikv_view* view, const void* q, 
     a.items = reinterpret_cast<ChunkItem*>(ws + 256);
     a.rec_o = reinterpret_cast<_Float16*>(ws + 256 + p.item_bytes);
     a.rec_ml = reinterpret_cast<float2*>(ws + 256 + p.item_bytes + p.o_bytes);
+    a.most_steps = p.steps;
+    a.tiles = reinterpret_cast<const half8*>(ws + 256 + p.item_bytes + p.o_bytes + p.ml_bytes);
     const bool kf = mode_k_f16(view->quant_mode), vf = mode_v_f16(view->quant_mode);
     hipStream_t s = static_cast<hipStream_t>(stream);
     return view->head_dim == 128 ? launch_chunk<128>(a, p, kf, vf, s) : launch_chunk<256>(a, p, kf, vf, s);
