@@ -27,7 +27,8 @@ namespace {
 
 constexpr uint32_t kSelectThreads = 1024;
 constexpr uint32_t kSelectWaves = kSelectThreads / 64;
-constexpr uint32_t kCopies = 16;    // histograms, one per lane % 16: weights share their top digits
+constexpr uint32_t kCopies = 16;  // histograms, one per lane % 16: weights share their top digits
+constexpr uint32_t kCopyStride = kCopies + 1;  // words from a digit's counts to the next one's; odd, for the sums' reads
 constexpr uint32_t kMoveTokens = 256;     // destination tokens moved at a time
 
 struct EvictArgs {
@@ -48,6 +49,11 @@ struct EvictArgs {
 
 __device__ __forceinline__ uint32_t evict_length(const EvictArgs& a, uint32_t b) { return min(a.lengths[b], a.max_context); }
 
+// Set bits of `mask` below this lane.
+__device__ __forceinline__ uint32_t lanes_before(unsigned long long mask) {
+    return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0u));
+}
+
 // Weights in the order of unsigned numbers; a NaN counts as less than any number.
 __device__ __forceinline__ uint32_t ordered(float w) {
     if (w != w) return 0u;
@@ -55,118 +61,155 @@ __device__ __forceinline__ uint32_t ordered(float w) {
     return (u & 0x80000000u) != 0 ? ~u : u | 0x80000000u;
 }
 
+// One workgroup of a (sequence, kv head).  Its keys lie in registers, kPer of each thread, a wave's
+// kPer * 64 one behind another: a context of up to kSegment keys between the first and the last ones
+// is read once, a longer one segment by segment in every pass.  Places behind the context count as
+// key 0, the least there is: they come last of all and more keys than stay are real, so none is chosen.
+//
+// Bound: instructions of one compute unit, 256 cycles for each one that every key of 16384 needs,
+// and the latency of the two reads and the barriers.  (For 16384 keys of 8 heads: the weights read anew
+// in every pass, one at a time, 31.4 us; held in registers 19; so 12.8.)
+constexpr uint32_t kPer = 16;
+constexpr uint32_t kSegment = kPer * kSelectThreads;
+
+__device__ __forceinline__ void load_weights(const float* w, uint32_t first, uint32_t hi, float (&x)[kPer], uint32_t (&key)[kPer]) {
+#pragma unroll
+    for (uint32_t j = 0; j < kPer; ++j) x[j] = w[min(first + j * 64, hi - 1)];
+#pragma unroll
+    for (uint32_t j = 0; j < kPer; ++j) key[j] = first + j * 64 < hi ? ordered(x[j]) : 0u;
+}
+
+// Sum over the lanes up to this one.
+__device__ __forceinline__ uint32_t sum_to_lane(uint32_t x) {
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x111, 0xf, 0xf, true);  // row_shr:1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x142, 0xa, 0xf, true);  // row_bcast:15, to rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x143, 0xc, 0xf, true);  // row_bcast:31, to rows 2 and 3
+    return x;
+}
+
 __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictArgs a) {
-    const uint32_t h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t L = evict_length(a, b), n = a.budget;
     const size_t row = static_cast<size_t>(b) * a.g.kv_heads + h;
     const float* w = a.weights + row * a.weight_stride;
+    float* out = a.weights_out == nullptr ? nullptr : a.weights_out + row * a.weight_out_stride;
+    const bool moves = out != nullptr, same_row = out == w;
     int32_t* kept = a.kept + row * n;
-    const uint32_t left = min(L, n);  // keys that stay
-    __shared__ uint32_t s_hist[kCopies][256];
-    __shared__ uint32_t s_digit, s_need;
-    __shared__ uint32_t s_gt[kSelectWaves], s_eq[kSelectWaves];
     if (L <= n) {
         for (uint32_t i = tid; i < n; i += kSelectThreads) kept[i] = i < L ? static_cast<int32_t>(i) : -1;
-    } else {
-        const uint32_t lo = a.sinks, hi = L - a.recent, need = n - a.sinks - a.recent;
-        for (uint32_t i = tid; i < a.sinks; i += kSelectThreads) kept[i] = static_cast<int32_t>(i);
-        for (uint32_t i = tid; i < a.recent; i += kSelectThreads) kept[n - a.recent + i] = static_cast<int32_t>(hi + i);
-        if (need != 0) {  // and then hi - lo > need
-            uint32_t prefix = 0, mask = 0, k = need;
-            for (int shift = 24; shift >= 0; shift -= 8) {
-                for (uint32_t i = tid; i < kCopies * 256; i += kSelectThreads) (&s_hist[0][0])[i] = 0;
-                __syncthreads();
-                for (uint32_t i = lo + tid; i < hi; i += kSelectThreads) {
-                    const uint32_t u = ordered(w[i]);
-                    if ((u & mask) == prefix) atomicAdd(&s_hist[lane % kCopies][(u >> shift) & 255u], 1u);
-                }
-                __syncthreads();
-                if (tid < 256) {
-                    uint32_t sum = 0;
+        if (moves && !same_row)
+            for (uint32_t i = tid; i < L; i += kSelectThreads) out[i] = w[i];
+        return;
+    }
+    __shared__ uint32_t s_hist[4][256 * kCopyStride];  // [pass][digit][copy]: equal digits of a wave on kCopies banks
+    __shared__ uint32_t s_count[4][256];
+    __shared__ uint2 s_total[2][kSelectWaves];  // keys above and at the limit, of a wave; segments in turn
+    const uint32_t lo = a.sinks, hi = L - a.recent, need = n - a.sinks - a.recent;
+    for (uint32_t i = tid; i < a.sinks; i += kSelectThreads) {
+        kept[i] = static_cast<int32_t>(i);
+        if (moves && !same_row) out[i] = w[i];
+    }
+    for (uint32_t i = tid; i < a.recent; i += kSelectThreads) kept[n - a.recent + i] = static_cast<int32_t>(hi + i);
+    if (need != 0) {  // and then hi - lo > need
+        const uint32_t first = lo + wave * (kPer * 64) + lane;
+        float x[kPer];
+        uint32_t key[kPer];
+        const bool once = hi - lo <= kSegment;
+        for (uint32_t i = tid; i < 4 * 256 * kCopyStride; i += kSelectThreads) (&s_hist[0][0])[i] = 0;
+        load_weights(w, first, hi, x, key);
+        __syncthreads();
+        uint32_t prefix = 0, k = need;
 #pragma unroll
-                    for (uint32_t c = 0; c < kCopies; ++c) sum += s_hist[c][tid];
-                    s_hist[0][tid] = sum;
-                }
-                __syncthreads();
-                if (wave == 0) {  // lane l: digits 255 - 4l down to 252 - 4l
-                    uint32_t c[4], sum = 0;
+        for (uint32_t pass = 0; pass < 4; ++pass) {
+            const uint32_t shift = 24 - 8 * pass;
+            uint32_t* const hist = &s_hist[pass][lane % kCopies];
+            for (uint32_t from = 0; from < hi - lo; from += kSegment) {
+                if (!once) load_weights(w, first + from, hi, x, key);
 #pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) sum += c[j] = s_hist[0][255 - 4 * lane - j];
-                    uint32_t incl = sum;
-#pragma unroll
-                    for (uint32_t off = 1; off < 64; off <<= 1) {
-                        const uint32_t up = __shfl_up(incl, off, 64);
-                        if (lane >= off) incl += up;
-                    }
-                    uint32_t above = incl - sum;
-#pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) {
-                        if (above < k && k <= above + c[j]) {  // exactly one lane and digit
-                            s_digit = 255 - 4 * lane - j;
-                            s_need = k - above;
-                        }
-                        above += c[j];
-                    }
-                }
-                __syncthreads();
-                prefix |= s_digit << shift;
-                mask |= 255u << shift;
-                k = s_need;
-            }
-            // Keys above `prefix` stay, and the first k of those equal to it.
-            const uint32_t seg = ((hi - lo + kSelectWaves - 1) / kSelectWaves + 63) / 64 * 64;
-            const uint32_t from = min(lo + wave * seg, hi), to = min(from + seg, hi);
-            uint32_t gt = 0, eq = 0;
-            for (uint32_t i = from; i < to; i += 64) {
-                const uint32_t u = i + lane < to ? ordered(w[i + lane]) : 0u;
-                gt += static_cast<uint32_t>(__popcll(__ballot(i + lane < to && u > prefix)));
-                eq += static_cast<uint32_t>(__popcll(__ballot(i + lane < to && u == prefix)));
-            }
-            if (lane == 0) {
-                s_gt[wave] = gt;
-                s_eq[wave] = eq;
+                for (uint32_t j = 0; j < kPer; ++j)
+                    if (pass == 0 || key[j] >> ((shift + 8) & 31) == prefix)
+                        atomicAdd(hist + ((key[j] >> shift) & 255u) * kCopyStride, 1u);
             }
             __syncthreads();
-            uint32_t gt0 = 0, eq0 = 0;
-            for (uint32_t x = 0; x < wave; ++x) {
-                gt0 += s_gt[x];
-                eq0 += s_eq[x];
+            if (tid < 256) {
+                uint32_t sum = 0;
+#pragma unroll
+                for (uint32_t c = 0; c < kCopies; ++c) sum += s_hist[pass][tid * kCopyStride + c];
+                s_count[pass][tid] = sum;
             }
-            uint32_t at = lo + gt0 + min(eq0, k);
-            const unsigned long long below = (1ull << lane) - 1ull;
-            for (uint32_t i = from; i < to; i += 64) {
-                const bool live = i + lane < to;
-                const uint32_t u = live ? ordered(w[i + lane]) : 0u;
-                const bool same = live && u == prefix;
-                const unsigned long long eqs = __ballot(same);
-                const uint32_t rank = eq0 + static_cast<uint32_t>(__popcll(eqs & below));
-                const bool keep = live && (u > prefix || (same && rank < k));
-                const unsigned long long keeps = __ballot(keep);
-                if (keep) kept[at + static_cast<uint32_t>(__popcll(keeps & below))] = static_cast<int32_t>(i + lane);
-                at += static_cast<uint32_t>(__popcll(keeps));
-                eq0 += static_cast<uint32_t>(__popcll(eqs));
+            __syncthreads();
+            // Every wave finds the digit.  Lane l: digits 255 - 4l down to 252 - 4l.
+            uint32_t c[4], sum = 0, digit = 0, before = 0;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) sum += c[j] = s_count[pass][255 - 4 * lane - j];
+            uint32_t above = sum_to_lane(sum) - sum;
+            const bool mine = above < k && k <= above + sum;  // of exactly one lane
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                if (above < k) {
+                    digit = 255 - 4 * lane - j;
+                    before = above;
+                }
+                above += c[j];
+            }
+            const uint32_t from_lane = static_cast<uint32_t>(__builtin_ctzll(__ballot(mine)));
+            prefix = prefix << 8 | static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(digit), from_lane));
+            k -= static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(before), from_lane));
+        }
+        // Keys above `prefix` stay, and the first k of those equal to it.  In place, a weight's new
+        // position is at or before its old one, and its segment has been read whole by then.
+        uint32_t gt0 = 0, eq0 = 0;  // keys above and equal, of the segments before
+        for (uint32_t from = 0, turn = 0; from < hi - lo; from += kSegment, turn ^= 1) {
+            if (!once) load_weights(w, first + from, hi, x, key);
+            uint32_t gt = 0, eq = 0;
+#pragma unroll
+            for (uint32_t j = 0; j < kPer; ++j) {
+                gt += static_cast<uint32_t>(__popcll(__ballot(key[j] > prefix)));
+                eq += static_cast<uint32_t>(__popcll(__ballot(key[j] == prefix)));
+            }
+            if (lane == 0) s_total[turn][wave] = make_uint2(gt, eq);
+            __syncthreads();
+            const uint2 mine = s_total[turn][lane % kSelectWaves];
+            const uint32_t gi = sum_to_lane(lane < kSelectWaves ? mine.x : 0u), ei = sum_to_lane(lane < kSelectWaves ? mine.y : 0u);
+            uint32_t gt_at = gt0 + static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(gi), wave)) - gt;
+            uint32_t eq_at = eq0 + static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(ei), wave)) - eq;
+            gt0 += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(gi), 63));
+            eq0 += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(ei), 63));
+#pragma unroll
+            for (uint32_t j = 0; j < kPer; ++j) {
+                const unsigned long long gts = __ballot(key[j] > prefix), eqs = __ballot(key[j] == prefix);
+                if ((gts | eqs) != 0) {
+                    const uint32_t eq_mine = eq_at + lanes_before(eqs);
+                    const uint32_t to = a.sinks + gt_at + lanes_before(gts) + min(eq_mine, k);
+                    if (key[j] > prefix || (key[j] == prefix && eq_mine < k)) {
+                        kept[to] = static_cast<int32_t>(first + from + j * 64);
+                        if (moves) out[to] = x[j];
+                    }
+                    gt_at += static_cast<uint32_t>(__popcll(gts));
+                    eq_at += static_cast<uint32_t>(__popcll(eqs));
+                }
             }
         }
     }
-    if (a.weights_out == nullptr) return;
-    float* out = a.weights_out + row * a.weight_out_stride;
-    const bool same_row = out == w;
-    if (same_row && L <= n) return;
-    __syncthreads();  // the list is whole, and the weights have been read
-    for (uint32_t i0 = 0; i0 < left; i0 += kSelectThreads) {
+    if (!moves) return;
+    // The last keys' weights; in place they go forward in order, all of a turn read before any is written.
+    if (same_row) __syncthreads();
+    for (uint32_t i0 = 0; i0 < a.recent; i0 += kSelectThreads) {
         const uint32_t i = i0 + tid;
-        const float x = i < left ? w[kept[i]] : 0.0f;
+        const float y = i < a.recent ? w[hi + i] : 0.0f;
         if (same_row) {
             wait_vmem();
             __syncthreads();
         }
-        if (i < left) out[i] = x;
+        if (i < a.recent) out[n - a.recent + i] = y;
     }
     // in place: what stood behind the keys that stay is no weight of the keys to come
     if (same_row)
-        for (uint32_t i = left + tid; i < L; i += kSelectThreads) {
-            out[i] = 0.0f;
-        }
+        for (uint32_t i = n + tid; i < L; i += kSelectThreads) out[i] = 0.0f;
 }
 
 typedef unsigned int u4v __attribute__((ext_vector_type(4)));

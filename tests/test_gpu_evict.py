@@ -165,6 +165,32 @@ def test_evict_long(gpu):
     _check(cache, before, w, kept, [n], new, 30000, 4, 1000)
 
 
+@pytest.mark.parametrize("n,budget,sinks,recent", [(16390, 9000, 4, 2), (16391, 9000, 4, 2), (40001, 21000, 0, 5000),
+                                                   (40001, 39990, 7, 30000), (50000, 50, 25, 25), (33000, 32999, 0, 0)])
+@pytest.mark.parametrize("own_rows", [True, False])
+def test_evict_long_weights(gpu, n, budget, sinks, recent, own_rows):
+    """Long contexts whose weights move too, over themselves or to rows of another stride; ties among them."""
+    import miinfer_amd as m
+    rng = np.random.default_rng(n + budget)
+    hk, d, cap = 2, 128, 50048
+    cache = m.KvCache.contiguous(hk, d, cap)
+    fill(cache, gpu, rng, [n])
+    w = np.zeros((1, hk, cap), np.float32)
+    w[0, 0, :n] = rng.integers(0, 9, n)
+    w[0, 1, :n] = rng.random(n)
+    before = [_rows(cache, 0, n)]
+    dw = _dev(w, gpu)
+    out = dw if own_rows else torch.full((1, hk, budget + 3), 5.0, device=gpu)
+    lens = torch.tensor([n], dtype=torch.int32, device=gpu)
+    kept, new = m.evict(cache, dw, lens, budget=budget, sinks=sinks, recent=recent, weights_out=out)
+    _check(cache, before, w, kept, [n], new, budget, sinks, recent)
+    k = kept.cpu().numpy()
+    for h in range(hk):
+        got = out[0, h].cpu().numpy()
+        assert np.array_equal(got[:budget], w[0, h, k[0, h]])
+        assert np.all(got[budget:] == (0.0 if own_rows else 5.0))
+
+
 def test_evict_graph(gpu):
     """A captured eviction to other pages, replayed with other weights and lengths."""
     import miinfer_amd as m
