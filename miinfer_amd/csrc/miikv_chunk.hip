@@ -39,6 +39,7 @@ constexpr uint32_t kMinUnits = 12;            // units per workgroup, at least
 constexpr uint32_t kMaxParts = 256;           // one workgroup per CU
 constexpr uint32_t kTileItems = 2;            // items per (sequence, kv head) from which on keys are expanded first
 constexpr uint64_t kMaxTileBytes = 1ull << 30;
+constexpr uint32_t kStageBytes = 4096;        // of a wave, for rows on their way to and from memory
 constexpr float kSlack = 8.0f;                // the maximum may grow by this (log2) before sums are rescaled
 
 struct ChunkItem {
@@ -239,9 +240,11 @@ struct TileLds {
     static constexpr uint32_t k_units = D / 8 * kChunk;
     static constexpr uint32_t v_row = D;
     static constexpr uint32_t units = k_units + 4 * v_row;
-    static constexpr uint32_t bufs = D == 128 ? 8 : 4;
-    static constexpr uint32_t ops = units * 16 / 1024 / kChunkWaves;
-    static constexpr uint32_t bytes = bufs * units * 16;
+    static constexpr uint32_t wide = D == 128 ? 2 : 1;  // steps of a turn
+    static constexpr uint32_t places = 4;               // turns of the ring
+    static constexpr uint32_t step_ops = units * 16 / 1024 / kChunkWaves, ops = wide * step_ops;
+    static constexpr uint32_t bytes = places * wide * units * 16;
+    static_assert(wide * units * 16 >= kChunkWaves * kStageBytes, "a place holds the waves' stages");
 };
 
 // Tile of a step (counted among the steps that any token of the chunk sees, `all`) of (b, h).
@@ -345,8 +348,9 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
     using Raw = ChunkLds<D, KF16, VF16>;
     using Lds = typename std::conditional<TILES, TileLds<D>, Raw>::type;
     extern __shared__ __align__(16) uint8_t lds[];
-    constexpr uint32_t kTiles = TILES ? Lds::bufs : 2;
-    half8* const s_tile = reinterpret_cast<half8*>(lds);  // [kTiles]
+    constexpr uint32_t W = TILES ? TileLds<D>::wide : 1;         // steps of a turn
+    constexpr uint32_t kPlaces = TILES ? TileLds<D>::places : 2;  // turns whose tiles are held
+    half8* const s_tile = reinterpret_cast<half8*>(lds);  // [kPlaces][W]
     uint8_t* const s_raw = lds + 2 * Raw::units * 16;
     _Float16* const s_vsc = reinterpret_cast<_Float16*>(s_raw + Raw::bufs * Raw::raw);  // [2][NB][4][8]
     uint32_t* const s_first = reinterpret_cast<uint32_t*>(lds + Lds::bytes);  // [batch + 1]: items before sequence b
@@ -384,7 +388,7 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
             it.b = lo;
             it.rows0 = (i - s_first[lo]) * kRows;
             it.steps = span_of(a, chunk_of(a, lo), it.rows0).vis.steps();
-            mine = kItemCost + it.steps;
+            mine = kItemCost + (it.steps + W - 1) / W * W;
         }
         const uint32_t incl = scan_threads(mine, s_wave, total);
         if (i < items) {
@@ -396,7 +400,7 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
     }
     units = uniform(units);
     const uint32_t axis = units * geo.kv_heads;  // the host has seen that it fits 32 bits
-    const uint32_t quota = uniform(max(axis / a.parts + (axis % a.parts != 0 ? 1u : 0u), kMinUnits));
+    const uint32_t quota = uniform((max(axis / a.parts + (axis % a.parts != 0 ? 1u : 0u), kMinUnits) + W - 1) / W * W);  // whole turns
     if (tid == 0) {
         s_start[items] = units;
         if (blockIdx.x == 0) {
@@ -426,6 +430,7 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
         if (uniform(s_first[mid]) <= i) b = mid;
         else hi = mid;
     }
+    uint32_t place = 1;  // of the ring, that no wave reads at an item's end
     for (; at < end; ++i) {
         if (i == items) {  // the next kv head's first
             ++h;
@@ -450,12 +455,11 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
 
         // ---- this wave's rows
         const uint32_t r = wave * 32 + n;  // of the item
-        const bool row_live = r < span.rows;
         const uint32_t row = rows0 + min(r, span.rows - 1);
         const uint32_t tok = row / a.group, head = h * a.group + (row - tok * a.group);
         const uint32_t past = c.length + tok + 1 > c.tokens ? c.length + tok + 1 - c.tokens : 0u;
         const uint32_t low = a.window != 0 && past > a.window ? past - a.window : 0u;
-        const size_t row_at = (static_cast<size_t>(c.q0 + tok) * a.q_heads + head) * D;
+        const uint32_t row_index = (c.q0 + tok) * a.q_heads + head;  // of q and out; the host has seen that it fits 31 bits
         const bool wave_live = wave * 32 < span.rows;
         // of the wave's first and last row
         const uint32_t past_a = __builtin_amdgcn_readfirstlane(past), low_a = __builtin_amdgcn_readfirstlane(low);
@@ -515,14 +519,17 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
         };
         auto fetch = [&]() __attribute__((always_inline)) {
             if (run_left == 0) locate();
-            if constexpr (TILES) {
-                const uint32_t to = lds_offset(s_tile) + next % Lds::bufs * Lds::units * 16 + wave * 1024;
+            if constexpr (TILES) {  // of one step
+                // (behind the last step of an odd number, that one again: its probabilities are 0)
+                const uint32_t to = lds_offset(s_tile) + (next - s0) % (kPlaces * W) * Lds::units * 16 + wave * 1024;
 #pragma unroll
-                for (uint32_t x = 0; x < TileLds<D>::ops; ++x)
+                for (uint32_t x = 0; x < TileLds<D>::step_ops; ++x)
                     copy_to_lds_from(src[0] + x * kChunkWaves * 1024, lane * 16, to + x * kChunkWaves * 1024);
-                src[0] += Lds::units * 16;
+                if (next + 1 < s1) {
+                    src[0] += Lds::units * 16;
+                    --run_left;
+                }
                 ++next;
-                --run_left;
                 return;
             }
             const uint32_t to = lds_offset(s_raw) + next % Raw::bufs * Raw::raw;
@@ -620,10 +627,6 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
 
         float m_run = -INFINITY, l_run = 0.0f;
         float16v O[NB];
-#pragma unroll
-        for (uint32_t mt = 0; mt < NB; ++mt)
-#pragma unroll
-            for (uint32_t x = 0; x < 16; ++x) O[mt][x] = 0.0f;
 
         // Whether this wave's rows see anything of a step (wave-uniform).
         auto seen = [&](uint32_t s) __attribute__((always_inline)) {
@@ -631,48 +634,57 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
             return wave_live & (tok0 < past_z) & ((a.window == 0) | (tok0 + kChunk > low_a) | (tok0 < a.sinks));
         };
         half8 qf[NQ];
-        float16v S;
-        half8 P[2];
-        // O^T += V^T P^T of step s - 1 (VALUES), then S^T = K Q^T of step s (SCORES): one run of MFMAs
+        float16v S[W];
+        half8 P[2 * W];
+        // O^T += V^T P^T of turn j - 1 (VALUES), then S^T = K Q^T of turn j (SCORES): one run of MFMAs
         // whose fragments are read kAhead ahead.
-        auto multiply = [&](auto with_values, auto with_scores, uint32_t s) __attribute__((always_inline)) {
-            constexpr uint32_t NV = decltype(with_values)::value ? 2 * NB : 0, N = NV + (decltype(with_scores)::value ? NQ : 0);
-            // value fragment c: dims 32 (c / 2) .., keys of units 2 (c % 2) + hh; key fragment: dims 16 c + 8 hh ..
-            const half8* v = s_tile + (s - 1) % kTiles * Lds::units + Lds::k_units + hh * Lds::v_row + n;
-            const half8* k = s_tile + s % kTiles * Lds::units + hh * kChunk + n;
+        auto multiply = [&](auto with_values, auto with_scores, uint32_t j) __attribute__((always_inline)) {
+            constexpr uint32_t NV = decltype(with_values)::value ? 2 * NB * W : 0, N = NV + (decltype(with_scores)::value ? NQ * W : 0);
+            // value fragment c of a step: dims 32 (c / 2) .., keys of units 2 (c % 2) + hh; key fragment: dims 16 c + 8 hh ..
+            const half8* v = s_tile + (j - 1) % kPlaces * W * Lds::units + Lds::k_units + hh * Lds::v_row + n;
+            const half8* k = s_tile + j % kPlaces * W * Lds::units + hh * kChunk + n;
             auto at = [&](uint32_t c) __attribute__((always_inline)) {
-                return c < NV ? v[c / 2 * kChunk + c % 2 * 2 * Lds::v_row] : k[(c - NV) * 2 * kChunk];
+                return c < NV ? v[c / (2 * NB) * Lds::units + c % (2 * NB) / 2 * kChunk + c % 2 * 2 * Lds::v_row]
+                              : k[(c - NV) / NQ * Lds::units + (c - NV) % NQ * 2 * kChunk];
             };
             half8 f[kAhead];
 #pragma unroll
             for (uint32_t c = 0; c < kAhead; ++c) f[c] = at(c);
             if constexpr (decltype(with_scores)::value)
 #pragma unroll
-                for (uint32_t x = 0; x < 16; ++x) S[x] = 0.0f;
+                for (uint32_t u = 0; u < W; ++u)
+#pragma unroll
+                    for (uint32_t x = 0; x < 16; ++x) S[u][x] = 0.0f;
             __builtin_amdgcn_sched_barrier(0);  // the scheduler would move reads to their use, or all of them up here
 #pragma unroll
             for (uint32_t c = 0; c < N; ++c) {
-                if (c < NV) O[c / 2] = mfma_32x32x16(f[c % kAhead], P[c % 2], O[c / 2]);
-                else S = mfma_32x32x16(f[c % kAhead], qf[c - NV], S);
+                if (c < NV) O[c % (2 * NB) / 2] = mfma_32x32x16(f[c % kAhead], P[c / (2 * NB) * 2 + c % 2], O[c % (2 * NB) / 2]);
+                else S[(c - NV) / NQ] = mfma_32x32x16(f[c % kAhead], qf[(c - NV) % NQ], S[(c - NV) / NQ]);
                 if (c + kAhead < N) f[c % kAhead] = at(c + kAhead);
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
         const std::true_type yes{};
         const std::false_type no{};
+        // Of the turn whose first step is s.
         auto softmax = [&](uint32_t s) __attribute__((always_inline)) {
-            const uint32_t tok0 = uniform(span.vis.step(s) * kChunk);
-            const bool whole = (tok0 + kChunk <= past_a) & ((a.window == 0) | (tok0 + kChunk <= a.sinks) | (tok0 >= low_z));
-            if (!whole) {
+            float top = -INFINITY;
 #pragma unroll
-                for (uint32_t x = 0; x < 16; ++x) {
-                    const uint32_t t = tok0 + 8 * (x / 4) + 4 * hh + x % 4;
-                    S[x] = (t >= past) | ((t < low) & (t >= a.sinks)) ? -INFINITY : S[x];
+            for (uint32_t u = 0; u < W; ++u) {
+                const uint32_t tok0 = uniform(span.vis.step(s + u) * kChunk);
+                const bool there = W == 1 || s + u < s1;
+                const bool whole = there & (tok0 + kChunk <= past_a) & ((a.window == 0) | (tok0 + kChunk <= a.sinks) | (tok0 >= low_z));
+                if (!whole) {
+#pragma unroll
+                    for (uint32_t x = 0; x < 16; ++x) {
+                        const uint32_t t = tok0 + 8 * (x / 4) + 4 * hh + x % 4;
+                        S[u][x] = !there | (t >= past) | ((t < low) & (t >= a.sinks)) ? -INFINITY : S[u][x];
+                    }
                 }
+                // (fmaxf would first quieten each of its inputs)
+                top = max3(top, max3(max3(S[u][0], S[u][1], S[u][2]), max3(S[u][3], S[u][4], S[u][5]), max3(S[u][6], S[u][7], S[u][8])),
+                           max3(max3(S[u][9], S[u][10], S[u][11]), max3(S[u][12], S[u][13], S[u][14]), S[u][15]));
             }
-            // (fmaxf would first quieten each of its inputs)
-            float top = max3(max3(max3(S[0], S[1], S[2]), max3(S[3], S[4], S[5]), max3(S[6], S[7], S[8])),
-                             max3(S[9], S[10], S[11]), max3(S[12], S[13], max3(S[14], S[15], S[15])));
             top = swap32_reduce(top, MaxOp{}) * a.scale_log2;
             if (__any(top > m_run + kSlack)) {
                 const float to = fmaxf(m_run, top);
@@ -683,27 +695,56 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
                 for (uint32_t mt = 0; mt < NB; ++mt) O[mt] *= f;
             }
             const float use = m_run == -INFINITY ? 0.0f : m_run;
-#pragma unroll
-            for (uint32_t x = 0; x < 16; ++x)
-                P[x / 4 % 2][x % 4 + x / 8 * 4] = static_cast<_Float16>(exp2_fast(fmaf(S[x], a.scale_log2, -use)));
-            // the sum of the probabilities as the second product takes them
+            // and the sum of the probabilities as the second product takes them
             const half2v one = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
-            float sum[2] = {0.0f, 0.0f};
+            float sum[2 * W] = {};
 #pragma unroll
-            for (uint32_t x = 0; x < 8; x += 2)
+            for (uint32_t u = 0; u < W; ++u) {
 #pragma unroll
-                for (uint32_t u = 0; u < 2; ++u) sum[u] = __builtin_amdgcn_fdot2(half2v{P[u][x], P[u][x + 1]}, one, sum[u], false);
-            l_run += sum[0] + sum[1];
+                for (uint32_t x = 0; x < 16; ++x)
+                    P[2 * u + x / 4 % 2][x % 4 + x / 8 * 4] = static_cast<_Float16>(exp2_fast(fmaf(S[u][x], a.scale_log2, -use)));
+#pragma unroll
+                for (uint32_t x = 0; x < 8; x += 2)
+#pragma unroll
+                    for (uint32_t y = 2 * u; y < 2 * u + 2; ++y) sum[y] = __builtin_amdgcn_fdot2(half2v{P[y][x], P[y][x + 1]}, one, sum[y], false);
+            }
+#pragma unroll
+            for (uint32_t y = 0; y < 2 * W; y += 2) l_run += sum[y] + sum[y + 1];
         };
         if (s0 < s1) {
             lds_barrier();  // the previous item's tiles and ring have been read
-            // (the query is waited for behind these: of tiles, no more than the first two steps)
-            for (uint32_t i = s0; i < min(s0 + (TILES ? 2 : Lds::bufs), s1); ++i) fetch();
+            // (the query is waited for behind these: of tiles, no more than the first two turns)
+            if constexpr (TILES) {
+                for (uint32_t i = 0; i < 2 * W; ++i)
+                    if (s0 + i / W * W < s1) fetch();
+            } else {
+                for (uint32_t i = s0; i < min(s0 + Raw::bufs, s1); ++i) fetch();
+            }
         }
-        with_type(a.q_dtype, [&](auto t) __attribute__((always_inline)) {
+        // The query comes row by row, each wave's through LDS of its own where no tile is yet.  (Fragments
+        // read straight from memory touch a line in each of 32 rows at a time.)
+        if (s0 < s1)
+            with_type(a.q_dtype, [&](auto t) __attribute__((always_inline)) {
+                const uint32_t me = here() % 64, mn = me % 32, mh = me / 32;
+                half8* const stage = s_tile + (TILES ? (kPlaces - 1) * W * Lds::units : 0) + wave * (kStageBytes / 16);
 #pragma unroll
-            for (uint32_t k = 0; k < NQ; ++k) qf[k] = load_query<decltype(t)>(a.q, row_at + 16 * k + 8 * hh);
-        });
+                for (uint32_t d0 = 0; d0 < D; d0 += 128) {
+                    half8 x[4][2];
+#pragma unroll
+                    for (uint32_t p = 0; p < 4; ++p) {
+                        const size_t at = static_cast<size_t>(__shfl(static_cast<int>(row_index), 8 * p + me / 8, 64)) * D + d0 + 8 * (me % 8);
+                        x[p][0] = load_query<decltype(t)>(a.q, at);
+                        x[p][1] = load_query<decltype(t)>(a.q, at + 64);
+                    }
+#pragma unroll
+                    for (uint32_t e = 0; e < 2; ++e) {
+#pragma unroll
+                        for (uint32_t p = 0; p < 4; ++p) stage[(8 * p + me / 8) * 8 + (me % 8 ^ me / 8)] = x[p][e];
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k) qf[d0 / 16 + 4 * e + k] = stage[mn * 8 + ((2 * k + mh) ^ (mn % 8))];
+                    }
+                }
+            });
         if (a.negate)
 #pragma unroll
             for (uint32_t k = 0; k < NQ; ++k) qf[k] = -qf[k];
@@ -712,11 +753,17 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
 #pragma unroll
         for (uint32_t k = 0; k < NQ; ++k) asm volatile("" : "+v"(qf[k]));
 
+#pragma unroll
+        for (uint32_t mt = 0; mt < NB; ++mt)
+#pragma unroll
+            for (uint32_t x = 0; x < 16; ++x) O[mt][x] = 0.0f;
+
         if (s0 < s1) {
             wait_vmem();
             lds_barrier();
             if constexpr (TILES) {
-                for (uint32_t i = s0 + 2; i < min(s0 + Lds::bufs, s1); ++i) fetch();
+                for (uint32_t i = 2 * W; i < kPlaces * W; ++i)
+                    if (s0 + i / W * W < s1) fetch();
             } else {
                 order_scales(s0);
                 if (!Raw::turns && s0 + 1 < s1) order_scales(s0 + 1);
@@ -726,28 +773,31 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
             }
         }
         if constexpr (TILES) {
-            // The two waves of a SIMD take turns: while waves 0..3 multiply (values of step s - 1, scores of
-            // step s), waves 4..7 do the softmax of step s - 1, and the other way round.  With
-            // t = s - s0, the first half multiplies in interval 2t and computes in 2t + 1, the second half
-            // one interval later.  Step s is read from 2t to 2t + 3 and must have landed before 2t; its
-            // place is fetched into anew from 2t + 4 on, in the turns of step s + 2.
+            // The two waves of a SIMD take turns of W steps: while waves 0..3 multiply (values of turn j - 1,
+            // scores of turn j), waves 4..7 do the softmax of turn j - 1, and the other way round.
+            // The first half multiplies in interval 2j and computes in 2j + 1, the second half one
+            // interval later.  Turn j is read from 2j to 2j + 3 and must have landed before 2j; its
+            // place is fetched into anew from 2j + 4 on, in the intervals of turn j + 2.
             const bool second = wave >= 4;
-            auto steps_of = [&](auto live) __attribute__((always_inline)) {
+            const uint32_t turns = (s1 - s0 + W - 1) / W;
+            auto turns_of = [&](auto live) __attribute__((always_inline)) {
                 constexpr bool kLive = decltype(live)::value;
                 if (second) lds_barrier();
-                if constexpr (kLive) multiply(no, yes, s0);
+                if constexpr (kLive) multiply(no, yes, 0);
                 // (The last pass multiplies scores that nothing uses: leaving the loop in front of them would
                 // hold the accumulators twice.)
-                for (uint32_t s = s0; s < s1; ++s) {
-                    if (second) {  // step s + 1 has landed
-                        if (s + Lds::bufs - 3 < s1) wait_vmem_le<(Lds::bufs - 4) * TileLds<D>::ops>();
+                for (uint32_t j = 0; j < turns; ++j) {
+                    if (second) {  // turn j + 1 has landed
+                        if (j + kPlaces - 3 < turns) wait_vmem_le<(kPlaces - 4) * TileLds<D>::ops>();
                         else wait_vmem();
                     }
                     lds_barrier();
-                    if (s >= s0 + 2 && s + Lds::bufs - 2 < s1) fetch();  // step s + bufs - 2
-                    if constexpr (kLive) softmax(s);
+                    if (j >= 2 && j + kPlaces - 2 < turns)  // turn j + 2
+#pragma unroll
+                        for (uint32_t u = 0; u < W; ++u) fetch();
+                    if constexpr (kLive) softmax(s0 + j * W);
                     if (!second) {
-                        if (s + Lds::bufs - 2 < s1) wait_vmem_le<(Lds::bufs - 3) * TileLds<D>::ops>();
+                        if (j + kPlaces - 2 < turns) wait_vmem_le<(kPlaces - 3) * TileLds<D>::ops>();
                         else wait_vmem();
                     }
                     // (the exponentials would move behind the barrier, into the turn that multiplies)
@@ -755,15 +805,16 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
                     lds_barrier();
                     if constexpr (kLive) {
                         __builtin_amdgcn_s_setprio(1);
-                        multiply(yes, yes, s + 1);
+                        multiply(yes, yes, j + 1);
                         __builtin_amdgcn_s_setprio(0);
                     }
                 }
                 if (!second) lds_barrier();
             };
             if (s0 < s1) {
-                if (wave_live) steps_of(yes);
-                else steps_of(no);
+                if (wave_live) turns_of(yes);
+                else turns_of(no);
+                place = (turns + 1) % kPlaces;
             }
         } else if constexpr (Raw::turns) {
             // The two waves of a SIMD take turns: while waves 0..3 multiply (values of step s - 1, scores
@@ -838,28 +889,42 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
         }
         l_run = swap32_reduce(l_run, AddOp{});
         const float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;  // a token that sees no key: zeros
-        if (s1 - s0 == steps) {
-            if (row_live)
-                with_type(a.out_dtype, [&](auto t) __attribute__((always_inline)) {
+        // Out row by row, through LDS that no wave reads any more: of a ring of tiles the place behind the
+        // scores that nothing uses, else the ring of codes.
+        uint8_t* const stage = (TILES ? lds + place * W * Lds::units * 16 : s_raw) + wave * kStageBytes;
+        auto put = [&](auto t, void* to, bool whole) __attribute__((always_inline)) {
+            const uint32_t me = here() % 64, mn = me % 32, mh = me / 32;
+            using T = decltype(t);
+            typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+            typedef T vec4 __attribute__((ext_vector_type(4)));
+            constexpr uint32_t kDims = 128 / sizeof(T);  // 128 bytes of each row at a time
+            const size_t rec = static_cast<size_t>(2 * part + (first < begin ? 0u : 1u)) * kRows + wave * 32;
 #pragma unroll
-                    for (uint32_t mt = 0; mt < NB; ++mt)
+            for (uint32_t d0 = 0; d0 < D; d0 += kDims) {
 #pragma unroll
-                        for (uint32_t x = 0; x < 16; x += 4)
-                            store4<decltype(t)>(a.out, row_at + 32 * mt + 2 * x + 4 * hh,
-                                                make_float4(O[mt][x] * inv, O[mt][x + 1] * inv, O[mt][x + 2] * inv, O[mt][x + 3] * inv));
-                });
-        } else if (row_live) {
-            const size_t rec = (static_cast<size_t>(2 * part + (first < begin ? 0u : 1u)) * kRows + r);
-#pragma unroll
-            for (uint32_t mt = 0; mt < NB; ++mt)
-#pragma unroll
-                for (uint32_t x = 0; x < 4; ++x) {
-                    half4 o;
-#pragma unroll
-                    for (uint32_t y = 0; y < 4; ++y) o[y] = static_cast<_Float16>(O[mt][4 * x + y] * inv);
-                    *reinterpret_cast<half4*>(a.rec_o + rec * D + 32 * mt + 8 * x + 4 * hh) = o;
+                for (uint32_t d = 0; d < kDims; d += 8) {  // this lane's 4 of 8
+                    const uint32_t mt = (d0 + d) / 32, x = (d0 + d) % 32 / 2, byte = (d + 4 * mh) * sizeof(T);
+                    *reinterpret_cast<vec4*>(stage + mn * 128 + ((byte / 16 ^ mn % 8) * 16) + byte % 16) =
+                        vec4{static_cast<T>(O[mt][x] * inv), static_cast<T>(O[mt][x + 1] * inv), static_cast<T>(O[mt][x + 2] * inv), static_cast<T>(O[mt][x + 3] * inv)};
                 }
-            if (hh == 0) a.rec_ml[rec] = make_float2(m_run, l_run);
+#pragma unroll
+                for (uint32_t p = 0; p < 4; ++p) {
+                    const uint32_t y = 8 * p + me / 8;
+                    const vec v = *reinterpret_cast<const vec*>(stage + y * 128 + (me % 8 ^ me / 8) * 16);
+                    const size_t at = whole ? static_cast<size_t>(__shfl(static_cast<int>(row_index), y, 64)) : rec + y;
+                    if (wave * 32 + y < span.rows)
+                        *reinterpret_cast<vec*>(static_cast<T*>(to) + at * D + d0 + me % 8 * (16 / sizeof(T))) = v;
+                }
+            }
+        };
+        if (!wave_live) continue;
+        if (s1 - s0 == steps) {
+            with_type(a.out_dtype, [&](auto t) __attribute__((always_inline)) { put(t, a.out, true); });
+        } else {
+            put(_Float16{}, a.rec_o, false);
+            const uint32_t me = here() % 64, y = wave * 32 + me % 32;
+            if ((me < 32) & (y < span.rows))
+                a.rec_ml[static_cast<size_t>(2 * part + (first < begin ? 0u : 1u)) * kRows + y] = make_float2(m_run, l_run);
         }
     }
 }
@@ -880,25 +945,42 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs a) {
     const Chunk c = chunk_of(a, it.b);
     if (it.rows0 + r >= c.tokens * a.group) return;
     const uint32_t tok = (it.rows0 + r) / a.group, head = h * a.group + (it.rows0 + r) % a.group;
-    float m = -INFINITY;
-    for (uint32_t w = w0; w <= w1; ++w) {
-        const size_t rec = static_cast<size_t>(2 * w + (first < w * quota ? 0u : 1u)) * kRows + r;
-        m = fmaxf(m, a.rec_ml[rec].x);
-    }
     constexpr uint32_t kPer = D / 64;  // groups of 8 values per thread
+    constexpr uint32_t kDepth = 4;     // records read at a time
     float acc[kPer][8] = {};
-    float sum = 0.0f;
-    for (uint32_t w = w0; w <= w1; ++w) {
-        const size_t rec = static_cast<size_t>(2 * w + (first < w * quota ? 0u : 1u)) * kRows + r;
-        const float2 ml = a.rec_ml[rec];
-        const float f = ml.x == -INFINITY ? 0.0f : ml.y * exp2_fast(ml.x - m);
-        sum += f;
+    float m = -INFINITY, sum = 0.0f;
+    for (uint32_t w = w0; w <= w1; w += kDepth) {
+        float2 ml[kDepth];
+        half8 o[kDepth][kPer];
 #pragma unroll
-        for (uint32_t k = 0; k < kPer; ++k) {
-            const half8 o = *reinterpret_cast<const half8*>(a.rec_o + rec * D + 64 * k + 8 * (threadIdx.x % 8));
+        for (uint32_t j = 0; j < kDepth; ++j) {
+            const uint32_t x = min(w + j, w1);
+            const size_t rec = static_cast<size_t>(2 * x + (first < x * quota ? 0u : 1u)) * kRows + r;
+            ml[j] = a.rec_ml[rec];
+            if (w + j > w1) ml[j] = make_float2(-INFINITY, 0.0f);
 #pragma unroll
-            for (uint32_t x = 0; x < 8; ++x) acc[k][x] = fmaf(static_cast<float>(o[x]), f, acc[k][x]);
+            for (uint32_t k = 0; k < kPer; ++k) o[j][k] = *reinterpret_cast<const half8*>(a.rec_o + rec * D + 64 * k + 8 * (threadIdx.x % 8));
         }
+        float to = m;
+#pragma unroll
+        for (uint32_t j = 0; j < kDepth; ++j) to = fmaxf(to, ml[j].x);
+        const float keep = m == -INFINITY ? 0.0f : exp2_fast(m - to);
+        m = to;
+        sum *= keep;
+        float f[kDepth];
+#pragma unroll
+        for (uint32_t j = 0; j < kDepth; ++j) {
+            f[j] = ml[j].x == -INFINITY ? 0.0f : ml[j].y * exp2_fast(ml[j].x - m);
+            sum += f[j];
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kPer; ++k)
+#pragma unroll
+            for (uint32_t x = 0; x < 8; ++x) {
+                acc[k][x] *= keep;
+#pragma unroll
+                for (uint32_t j = 0; j < kDepth; ++j) acc[k][x] = fmaf(static_cast<float>(o[j][k][x]), f[j], acc[k][x]);
+            }
     }
     const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
     const size_t at = (static_cast<size_t>(c.q0 + tok) * a.q_heads + head) * D + 8 * (threadIdx.x % 8);
@@ -945,7 +1027,7 @@ int chunk_plan(const miikv_view* v, uint32_t q_heads, uint32_t batch, uint32_t t
     // every sequence's last item may be a part of one
     p.items = std::min<uint64_t>(rows / kRows + batch, rows);
     p.steps = most_visible_steps(max_context, max_tokens, window, sinks);
-    const uint64_t most = kItemCost + p.steps;
+    const uint64_t most = kItemCost + p.steps + 1;  // (whole turns)
     const uint64_t axis = p.items * most * v->kv_heads;
     if (axis / v->kv_heads / most != p.items || axis > 0xf0000000u) return MIIKV_EUNSUPPORTED;  // 32-bit places on the axis
     p.parts = static_cast<uint32_t>(std::min<uint64_t>(kMaxParts, (axis + kMinUnits - 1) / kMinUnits));
