@@ -34,7 +34,7 @@ namespace {
 constexpr uint32_t kChunkWaves = 8;
 constexpr uint32_t kChunkThreads = 64 * kChunkWaves;
 constexpr uint32_t kRows = 32 * kChunkWaves;  // rows of an item
-constexpr uint32_t kItemCost = 4;             // an item's fixed cost, in steps
+constexpr uint32_t kItemCost = 8;             // an item's fixed cost, in steps
 constexpr uint32_t kMinUnits = 12;            // units per workgroup, at least
 constexpr uint32_t kMaxParts = 256;           // one workgroup per CU
 constexpr uint32_t kTileItems = 2;            // items per (sequence, kv head) from which on keys are expanded first
@@ -47,6 +47,10 @@ struct ChunkItem {
     uint32_t rows0;  // its first row
     uint32_t start;  // units of one kv head before it
     uint32_t steps;
+    uint32_t rows;   // of it
+    uint32_t tok0;   // row0's token, in q
+    uint32_t head0;  // and query head of the group
+    uint32_t unused;
 };
 
 struct ChunkArgs {
@@ -387,7 +391,12 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
             }
             it.b = lo;
             it.rows0 = (i - s_first[lo]) * kRows;
-            it.steps = span_of(a, chunk_of(a, lo), it.rows0).vis.steps();
+            const Chunk c = chunk_of(a, lo);
+            const Span span = span_of(a, c, it.rows0);
+            it.steps = span.vis.steps();
+            it.rows = span.rows;
+            it.tok0 = c.q0 + it.rows0 / a.group;
+            it.head0 = it.rows0 % a.group;
             mine = kItemCost + (it.steps + W - 1) / W * W;
         }
         const uint32_t incl = scan_threads(mine, s_wave, total);
@@ -548,6 +557,12 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
             ++next;
             --run_left;
         };
+        // The item's first `count` steps (whole turns of tiles).
+        constexpr uint32_t kFirst = TILES ? W : Raw::turns ? 2 : Raw::landed + 1;
+        auto fetch_to = [&](uint32_t count) __attribute__((always_inline)) {
+            const uint32_t to = s0 + min(count, (s1 - s0 + W - 1) / W * W);
+            while (next < to) fetch();
+        };
         // Keys of the step that no row of the item sees may hold anything: their values are zeroed.
         auto unseen = [&](uint32_t t) __attribute__((always_inline)) {
             return (t >= span.past) | ((t < span.vis.lo) & (t >= a.sinks));
@@ -575,11 +590,10 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
         // A step's codes to fp16: each thread 16 codes of K and / or of V (D = 128: the first four
         // waves K's, the others V's).
         constexpr bool kBoth = D == 256;
-        auto convert_k = [&](uint32_t i) __attribute__((always_inline)) {
-            const uint32_t idx = here();
+        auto convert_k_run = [&](uint32_t i, uint32_t idx) __attribute__((always_inline)) {
             const uint8_t* raw = s_raw + i % Raw::bufs * Raw::raw;
             half8* tile = s_tile + (i & 1) * Raw::units;
-            if (kBoth || wave < 4) {
+            {
                 // key 16 T + m, dims 64 c + 8 g and 64 c + 32 + 8 g
                 const uint32_t T = idx / D, c = idx / 64 % (D / 64), g = idx / 16 % 4, m = idx % 16;
                 half8* to = tile + (8 * c + g) * kChunk + 16 * T + m;
@@ -595,11 +609,10 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
                 }
             }
         };
-        auto convert_v = [&](uint32_t i) __attribute__((always_inline)) {
-            const uint32_t idx = kBoth ? here() : here() & 255u;
+        auto convert_v_run = [&](uint32_t i, uint32_t idx) __attribute__((always_inline)) {
             const uint8_t* raw = s_raw + i % Raw::bufs * Raw::raw;
             half8* tile = s_tile + (i & 1) * Raw::units;
-            if (kBoth || wave >= 4) {
+            {
                 // dim d, keys of units 2x and 2x + 1
                 const uint32_t d = idx / 2, x = idx % 2;
                 half8* to = tile + Raw::k_units + 2 * x * Raw::v_row + d;
@@ -627,6 +640,13 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
 
         float m_run = -INFINITY, l_run = 0.0f;
         float16v O[NB];
+
+        auto convert_k = [&](uint32_t i) __attribute__((always_inline)) {
+            if (kBoth || wave < 4) convert_k_run(i, here());
+        };
+        auto convert_v = [&](uint32_t i) __attribute__((always_inline)) {
+            if (kBoth || wave >= 4) convert_v_run(i, kBoth ? here() : here() & 255u);
+        };
 
         // Whether this wave's rows see anything of a step (wave-uniform).
         auto seen = [&](uint32_t s) __attribute__((always_inline)) {
@@ -713,13 +733,8 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
         };
         if (s0 < s1) {
             lds_barrier();  // the previous item's tiles and ring have been read
-            // (the query is waited for behind these: of tiles, no more than the first two turns)
-            if constexpr (TILES) {
-                for (uint32_t i = 0; i < 2 * W; ++i)
-                    if (s0 + i / W * W < s1) fetch();
-            } else {
-                for (uint32_t i = s0; i < min(s0 + Raw::bufs, s1); ++i) fetch();
-            }
+            // no more than the first pass reads: the query is waited for behind these
+            fetch_to(kFirst);
         }
         // The query comes row by row, each wave's through LDS of its own where no tile is yet.  (Fragments
         // read straight from memory touch a line in each of 32 rows at a time.)
@@ -760,11 +775,12 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
 
         if (s0 < s1) {
             wait_vmem();
-            lds_barrier();
             if constexpr (TILES) {
-                for (uint32_t i = 2 * W; i < kPlaces * W; ++i)
-                    if (s0 + i / W * W < s1) fetch();
+                lds_barrier();
+                fetch_to(kPlaces * W);
             } else {
+                fetch_to(Raw::bufs);
+                lds_barrier();
                 order_scales(s0);
                 if (!Raw::turns && s0 + 1 < s1) order_scales(s0 + 1);
                 lds_barrier();
@@ -828,7 +844,10 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
             // A wave without rows only copies and converts.  (What a wave's rows do not see of the item's
             // steps is multiplied and masked: with a branch around it the accumulators would be held
             // twice.)
+            // Where the rows fill no wave of the second half, it converts all codes, K of step s + 1 in
+            // interval 2t and V of step s in 2t + 1.
             const bool second = wave >= 4;
+            const bool helped = span.rows <= kRows / 2;
             auto steps_of = [&](auto live) __attribute__((always_inline)) {
                 constexpr bool kLive = decltype(live)::value;
                 if (second) {
@@ -849,8 +868,10 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
                         if (s + 2 < s1) convert_k(s + 2);
                         if (s + 1 < s1) convert_v(s + 1);
                     } else {
-                        if (s + 1 < s1) convert_k(s + 1);
-                        convert_v(s);
+                        if (!helped) {
+                            if (s + 1 < s1) convert_k(s + 1);
+                            convert_v(s);
+                        }
                         if (s + 3 < s1) wait_vmem_le<Raw::ops>();  // step s + 2 has landed
                         else wait_vmem();
                     }
@@ -863,8 +884,25 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
                 }
                 if (!second) lds_barrier();
             };
+            auto help = [&]() __attribute__((always_inline)) {
+                constexpr uint32_t kRuns = kBoth ? 2 : 1;
+                lds_barrier();
+                for (uint32_t s = s0; s < s1; ++s) {
+                    if (s >= s0 + 2 && s + 2 < s1) fetch();  // step s + 2
+                    if (s + 1 < s1)
+#pragma unroll
+                        for (uint32_t x = 0; x < kRuns; ++x) convert_k_run(s + 1, (here() & 255u) + 256 * x);
+                    lds_barrier();
+#pragma unroll
+                    for (uint32_t x = 0; x < kRuns; ++x) convert_v_run(s, (here() & 255u) + 256 * x);
+                    wait_vmem();  // step s + 2 has landed
+                    lds_barrier();
+                }
+                lds_barrier();
+            };
             if (s0 < s1) {
-                if (wave_live) steps_of(yes);
+                if (helped & second) help();
+                else if (wave_live) steps_of(yes);
                 else steps_of(no);
             }
         } else {
@@ -934,17 +972,14 @@ constexpr uint32_t kMergeRows = 32;
 template <uint32_t D>
 __global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs a) {
     const uint32_t i = blockIdx.x / (kRows / kMergeRows), h = blockIdx.y;
-    if (i >= a.head[0]) return;
-    const ChunkItem it = a.items[i];
-    const uint32_t units = a.head[1], quota = a.head[2];
+    const uint32_t r = blockIdx.x % (kRows / kMergeRows) * kMergeRows + threadIdx.x / 8;
+    const ChunkItem it = a.items[i];  // (of nothing behind the last one: read with `head`, not after it)
+    const uint32_t items = a.head[0], units = a.head[1], quota = a.head[2];
+    if (i >= items || it.steps == 0 || r >= it.rows) return;
     const uint32_t first = h * units + it.start + kItemCost;
-    if (it.steps == 0) return;
     const uint32_t w0 = first / quota, w1 = (first + it.steps - 1) / quota;
     if (w0 == w1) return;  // written whole
-    const uint32_t r = blockIdx.x % (kRows / kMergeRows) * kMergeRows + threadIdx.x / 8;
-    const Chunk c = chunk_of(a, it.b);
-    if (it.rows0 + r >= c.tokens * a.group) return;
-    const uint32_t tok = (it.rows0 + r) / a.group, head = h * a.group + (it.rows0 + r) % a.group;
+    const uint32_t tok = it.tok0 + (it.head0 + r) / a.group, head = h * a.group + (it.head0 + r) % a.group;
     constexpr uint32_t kPer = D / 64;  // groups of 8 values per thread
     constexpr uint32_t kDepth = 4;     // records read at a time
     float acc[kPer][8] = {};
@@ -983,7 +1018,7 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs a) {
             }
     }
     const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-    const size_t at = (static_cast<size_t>(c.q0 + tok) * a.q_heads + head) * D + 8 * (threadIdx.x % 8);
+    const size_t at = (static_cast<size_t>(tok) * a.q_heads + head) * D + 8 * (threadIdx.x % 8);
     with_type(a.out_dtype, [&](auto t) __attribute__((always_inline)) {
 #pragma unroll
         for (uint32_t k = 0; k < kPer; ++k)
