@@ -8,7 +8,7 @@
 // Work.  The rows of a (sequence, kv head) are its (token, query head of the group) pairs;
 // kRows of them are an item, whose tokens together see a run of 32-key steps (and the steps
 // of the first tokens).  Items differ in length (short chunks, causality, windows), so the
-// items of all kv heads are laid on one axis, kItemCost units and one per step each, and the
+// items of all kv heads are laid on one axis, some units per item and per step, and the
 // axis is cut into equal parts, one per workgroup of the one resident round: every CU has the
 // same work whatever the lengths are.  An item that lies in one part is written straight
 // to the output; the parts of one that is cut leave records, which the second launch merges.
@@ -34,8 +34,12 @@ namespace {
 constexpr uint32_t kChunkWaves = 8;
 constexpr uint32_t kChunkThreads = 64 * kChunkWaves;
 constexpr uint32_t kRows = 32 * kChunkWaves;  // rows of an item
-constexpr uint32_t kItemCost = 8;             // an item's fixed cost, in steps
-constexpr uint32_t kMinUnits = 12;            // units per workgroup, at least
+// Units of the axis: of a step, of one whose codes are converted by waves without rows, and an item's fixed
+// cost (12 chunks of 40 and of 20 tokens over 9000 more keys, head_dim 256: 122 and 80 us more; prompts
+// with 4 and 8 steps as an item's cost: 180 and 165 us).
+constexpr uint32_t kStepCost = 3, kHelpedCost = 2;
+constexpr uint32_t kItemCost = 8 * kStepCost;
+constexpr uint32_t kMinUnits = 12 * kStepCost;  // per workgroup, at least
 constexpr uint32_t kMaxParts = 256;           // one workgroup per CU
 constexpr uint32_t kTileItems = 2;            // items per (sequence, kv head) from which on keys are expanded first
 constexpr uint64_t kMaxTileBytes = 1ull << 30;
@@ -50,7 +54,7 @@ struct ChunkItem {
     uint32_t rows;   // of it
     uint32_t tok0;   // row0's token, in q
     uint32_t head0;  // and query head of the group
-    uint32_t unused;
+    uint32_t last;   // axis places from its first turn to its last one
 };
 
 struct ChunkArgs {
@@ -366,6 +370,7 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
     const Geo& geo = a.g;
 
     // ---- the plan, by every workgroup for itself
+    auto turn_cost = [](uint32_t rows) { return W * (!TILES && Raw::turns && rows <= kRows / 2 ? kHelpedCost : kStepCost); };
     uint32_t base = 0, total;
     for (uint32_t b0 = 0; b0 < a.batch; b0 += kChunkThreads) {
         const uint32_t b = b0 + tid;
@@ -397,7 +402,9 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
             it.rows = span.rows;
             it.tok0 = c.q0 + it.rows0 / a.group;
             it.head0 = it.rows0 % a.group;
-            mine = kItemCost + (it.steps + W - 1) / W * W;
+            const uint32_t turns = (it.steps + W - 1) / W, cost = turn_cost(span.rows);
+            it.last = turns == 0 ? 0u : (turns - 1) * cost;
+            mine = kItemCost + turns * cost;
         }
         const uint32_t incl = scan_threads(mine, s_wave, total);
         if (i < items) {
@@ -409,7 +416,7 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
     }
     units = uniform(units);
     const uint32_t axis = units * geo.kv_heads;  // the host has seen that it fits 32 bits
-    const uint32_t quota = uniform((max(axis / a.parts + (axis % a.parts != 0 ? 1u : 0u), kMinUnits) + W - 1) / W * W);  // whole turns
+    const uint32_t quota = uniform(max(axis / a.parts + (axis % a.parts != 0 ? 1u : 0u), kMinUnits));
     if (tid == 0) {
         s_start[items] = units;
         if (blockIdx.x == 0) {
@@ -456,9 +463,12 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
         span.past = uniform(span.past);
         span.vis = {uniform(span.vis.head), uniform(span.vis.first), uniform(span.vis.end), uniform(span.vis.lo)};
         const uint32_t steps = span.vis.steps();
-        const uint32_t first = start + kItemCost;  // the axis place of its first step
-        const uint32_t s0 = uniform(at > first ? at - first : 0u);
-        const uint32_t s1 = uniform(end > first ? min(end - first, steps) : 0u);
+        const uint32_t first = start + kItemCost;  // the axis place of its first turn
+        // the turns that start within the part
+        const bool full = W * kStepCost == turn_cost(span.rows);
+        auto turns_to = [&](uint32_t x) { return full ? (x + W * kStepCost - 1) / (W * kStepCost) : (x + W * kHelpedCost - 1) / (W * kHelpedCost); };
+        const uint32_t s0 = uniform(at > first ? turns_to(at - first) * W : 0u);
+        const uint32_t s1 = uniform(end > first ? min(turns_to(end - first) * W, steps) : 0u);
         at = stop;
         if (s0 >= s1 && !(steps == 0 && start >= begin)) continue;  // only some of its fixed cost is here
 
@@ -977,7 +987,7 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs a) {
     const uint32_t items = a.head[0], units = a.head[1], quota = a.head[2];
     if (i >= items || it.steps == 0 || r >= it.rows) return;
     const uint32_t first = h * units + it.start + kItemCost;
-    const uint32_t w0 = first / quota, w1 = (first + it.steps - 1) / quota;
+    const uint32_t w0 = first / quota, w1 = (first + it.last) / quota;
     if (w0 == w1) return;  // written whole
     const uint32_t tok = it.tok0 + (it.head0 + r) / a.group, head = h * a.group + (it.head0 + r) % a.group;
     constexpr uint32_t kPer = D / 64;  // groups of 8 values per thread
@@ -1062,7 +1072,7 @@ int chunk_plan(const miikv_view* v, uint32_t q_heads, uint32_t batch, uint32_t t
     // every sequence's last item may be a part of one
     p.items = std::min<uint64_t>(rows / kRows + batch, rows);
     p.steps = most_visible_steps(max_context, max_tokens, window, sinks);
-    const uint64_t most = kItemCost + p.steps + 1;  // (whole turns)
+    const uint64_t most = kItemCost + (p.steps + 1ull) * kStepCost;  // (whole turns)
     const uint64_t axis = p.items * most * v->kv_heads;
     if (axis / v->kv_heads / most != p.items || axis > 0xf0000000u) return MIIKV_EUNSUPPORTED;  // 32-bit places on the axis
     p.parts = static_cast<uint32_t>(std::min<uint64_t>(kMaxParts, (axis + kMinUnits - 1) / kMinUnits));
