@@ -41,7 +41,12 @@ constexpr uint32_t kStepCost = 3, kHelpedCost = 2;
 constexpr uint32_t kItemCost = 8 * kStepCost;
 constexpr uint32_t kMinUnits = 12 * kStepCost;  // per workgroup, at least
 constexpr uint32_t kMaxParts = 256;           // one workgroup per CU
-constexpr uint32_t kTileItems = 2;            // items per (sequence, kv head) from which on keys are expanded first
+// Keys are expanded to fp16 tiles first from this many items per (sequence, kv head) on, of a call's
+// average: an expansion costs about the read and the write of the tiles, and saves its items' conversions.
+// (Four sequences of 8192 keys, us without and with: head_dim 128, 4 items 170 and 173, 8 items 316 and
+// 292; head_dim 256, 4 items 173 and 181, 8 items 284 and 275; fp16 planes 168 and 183, 312 and 300,
+// 199 and 189, 311 and 283.)
+constexpr uint32_t kTileItems = 6;
 constexpr uint64_t kMaxTileBytes = 1ull << 30;
 constexpr uint32_t kStageBytes = 4096;        // of a wave, for rows on their way to and from memory
 constexpr float kSlack = 8.0f;                // the maximum may grow by this (log2) before sums are rescaled

@@ -97,6 +97,55 @@ def test_chunk_groups(gpu, hq, hk, d):
         _check(cache, q, _call(gpu, cache, q, new, lengths, window=window, sinks=sinks), new, lengths, window, sinks)
 
 
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("mode", [0, 1, 2, 3])
+@pytest.mark.parametrize("window,sinks,page", [(0, 0, 64), (70, 0, 128), (33, 4, 64), (64, 130, 192), (1, 0, 64)])
+def test_chunk_many_rows(gpu, d, mode, window, sinks, page):
+    """Many rows of every sequence: prompts, odd and even numbers of steps, an empty chunk, a single token."""
+    rng = np.random.default_rng(d + mode + window)
+    new, lengths = [130, 0, 200, 1, 160], [130, 40, 500, 333, 193]
+    cache = paged(gpu, rng, 1, d, lengths, mode=mode, page=page)
+    q = _query(rng, gpu, (sum(new), 16, d), torch.bfloat16)
+    out = _call(gpu, cache, q, new, lengths, max_tokens=200, max_context=500, window=window, sinks=sinks)
+    _check(cache, q, out, new, lengths, window, sinks)
+
+
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("mode", [0, 3])
+def test_chunk_many_rows_masked_keys_and_cuts(gpu, d, mode):
+    """Many rows over a long context, whose items go over many workgroups; what no token sees may
+    hold anything, and pages that no token sees may be missing."""
+    rng = np.random.default_rng(d + mode)
+    n, t = 3005, 100
+    cache = paged(gpu, rng, 1, d, [n], mode=mode)
+    q = _query(rng, gpu, (t, 16, d), torch.float16)
+    for window, sinks in ((0, 0), (700, 5)):
+        out = _call(gpu, cache, q, [t], [n], window=window, sinks=sinks, max_context=cache.capacity)
+        _check(cache, q, out, [t], [n], window, sinks)
+    page = cache.block_table[0].long()
+    hidden = [j for j in range(3008) if not (n - t - window + 1 <= j < n or j < sinks)]
+    for name, shape in (("k_scales", (cache.num_pages, 1, 64, d // 32)), ("v_scales", (cache.num_pages, 1, 64, d // 32)),
+                        ("k_codes", (cache.num_pages, 1, 4, d // 64, 4, 16, 2, 8)),
+                        ("v_codes", (cache.num_pages, 1, 2, d, 4, 2, 4))):
+        x = getattr(cache, name)
+        if x is None or x.dtype == torch.int8:
+            continue
+        x = x.view(torch.float16).view(shape)
+        for i, j in enumerate(hidden):
+            bad, s, p = float("nan") if i % 2 else float("inf"), j % 64, page[j // 64]
+            if "scales" in name:
+                x[p, :, s] = bad
+            elif name == "k_codes":
+                x[p, :, s // 16, :, :, s % 16] = bad
+            else:
+                x[p, :, s // 32, :, s % 16 // 4, s % 32 // 16, s % 4] = bad
+    table = cache.block_table.clone()
+    table[0, 1:(n - t - window) // 64] = -1
+    cache.set_block_table(table)
+    got = _call(gpu, cache, q, [t], [n], window=window, sinks=sinks, max_context=cache.capacity)
+    assert torch.equal(got, out)
+
+
 def test_chunk_long_items_are_cut(gpu):
     """Few rows over a long context: an item's keys go over many workgroups; and types of query
     and output that differ."""
