@@ -16,8 +16,8 @@
 // and the probabilities (times V's block scale) as hi + lo fp16 parts too, 22 bits in all.
 // P enters 2^shift above its value, so that both parts of a probability of 2^-20 stay clear
 // of fp16's denormals: p <= 1 is multiplied by V's block scale, so shift is what the largest
-// scale so far leaves below 2^15 (scales of 0.02: shift 20; with 6, outputs were 3.6e-6
-// off instead of 4e-7).
+// scale so far leaves below 2^15 (values of 0.02: outputs 4.5e-7 off; with a shift of 6 they
+// were 3.4e-6 to 4.9e-6 off).
 //
 // Work: the visible 32-key steps of all sequences are cut into runs of 4 * cpw steps, one
 // workgroup (of four waves) each.  cpw is chosen on the device from the lengths, so that
@@ -580,38 +580,54 @@ __device__ void add_weights(const PartArgs& a, uint32_t x) {
     for (uint32_t c = 0; c < 16; ++c) s[c] = c < a.cols ? row[static_cast<size_t>(c) * a.logit_keys] : -INFINITY;
     float* to = a.weights + static_cast<size_t>(bh) * a.weight_stride + (live ? key : 0u);
     const float before = *to;
-    __shared__ float s_m[16][16], s_l[16][16];
+    // Thread (rg, c) folds records rg, rg + 16, ..; then the four of a wave meet in a fixed butterfly, and the waves.
+    __shared__ float s_m[kWaves][16], s_l[kWaves][16];
     const uint32_t c = threadIdx.x & 15, rg = threadIdx.x >> 4;
     uint32_t first, runs;
     find_records(a, bh, b, first, runs);
     const uint32_t rec = part_record(a.cols, D);
     float m = -INFINITY, l = 0.0f;
+    auto fold = [](float& m1, float& l1, float m2, float l2) {
+        const float mn = fmaxf(m1, m2);
+        l1 = l1 * (m1 == -INFINITY ? 0.0f : exp2_fast(m1 - mn)) + l2 * (m2 == -INFINITY ? 0.0f : exp2_fast(m2 - mn));
+        m1 = mn;
+    };
+    constexpr uint32_t kDepth = 4;  // records read at a time
     if (c < a.cols)
-        for (uint32_t r = rg; r < runs; r += 16) {
-            const float* p = a.part + static_cast<size_t>(first + r) * rec + a.cols * D;
-            const float m2 = p[c], l2 = p[a.cols + c];
-            const float mn = fmaxf(m, m2);
-            l = l * (m == -INFINITY ? 0.0f : exp2_fast(m - mn)) + l2 * (m2 == -INFINITY ? 0.0f : exp2_fast(m2 - mn));
-            m = mn;
+        for (uint32_t r = rg; r < runs; r += 16 * kDepth) {
+            float ms[kDepth], ls[kDepth];
+#pragma unroll
+            for (uint32_t j = 0; j < kDepth; ++j) {
+                const float* p = a.part + static_cast<size_t>(first + min(r + 16 * j, runs - 1)) * rec + a.cols * D;
+                ms[j] = p[c];
+                ls[j] = p[a.cols + c];
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < kDepth; ++j)
+                if (r + 16 * j < runs) fold(m, l, ms[j], ls[j]);
         }
-    s_m[rg][c] = m;
-    s_l[rg][c] = l;
+#pragma unroll
+    for (uint32_t off = 16; off < 64; off <<= 1) {
+        const float m2 = __shfl_xor(m, off), l2 = __shfl_xor(l, off);
+        fold(m, l, m2, l2);
+    }
+    if (threadIdx.x % 64 < 16) {
+        s_m[threadIdx.x / 64][c] = m;
+        s_l[threadIdx.x / 64][c] = l;
+    }
     __syncthreads();
+    __shared__ float s_ref[16], s_inv[16];
     if (threadIdx.x < 16) {
-        for (uint32_t r = 1; r < 16; ++r) {
-            const float m2 = s_m[r][c], l2 = s_l[r][c];
-            const float mn = fmaxf(m, m2);
-            l = l * (m == -INFINITY ? 0.0f : exp2_fast(m - mn)) + l2 * (m2 == -INFINITY ? 0.0f : exp2_fast(m2 - mn));
-            m = mn;
-        }
-        s_m[0][c] = m == -INFINITY ? 0.0f : m;
-        s_l[0][c] = l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+        for (uint32_t w = 1; w < kWaves; ++w) fold(m, l, s_m[w][c], s_l[w][c]);
+        s_ref[c] = m == -INFINITY ? 0.0f : m;
+        s_inv[c] = l > 0.0f ? 1.0f / l : 0.0f;
     }
     __syncthreads();
     float sum = 0.0f;
 #pragma unroll
     for (uint32_t k = 0; k < 16; ++k)
-        if (k < a.cols) sum += exp2_fast(s[k] - s_m[0][k]) * s_l[0][k];
+        if (k < a.cols) sum += exp2_fast(s[k] - s_ref[k]) * s_inv[k];
     if (live) *to = before + sum;
 }
 
