@@ -389,10 +389,13 @@ miikv_status miikv_suffix_attn_ex(const miikv_view* view, const uint16_t* k_new,
  *        (or total_tokens) is left out.
  * Precision: query, dequantised keys and values, and probabilities are rounded to fp16
  * once, sums and statistics are fp32 (about 4e-4 of the outputs' norm; an fp32 out shows
- * it).  A value that is not finite spreads to the call's tokens that see another key of
- * its 32-key step.  miikv_chunk_workspace_bytes() is 0 for arguments that the call
- * refuses; MIIKV_EUNSUPPORTED for batches whose plan does not fit a workgroup's LDS
- * (about 16000 items of 256 (token, query head) rows). */
+ * it).  A value that is not finite, in a key that some token of a chunk sees, may spread
+ * to the chunk's other tokens; what no token sees may hold anything.
+ * Workspace: miikv_chunk_workspace_bytes(), 0 for arguments that the call refuses.  It
+ * grows with max_tokens and max_context: where rows are many, keys are expanded to fp16
+ * in it first (1 GiB at most).  It needs no initialisation; calls that may overlap need
+ * workspaces of their own.  MIIKV_EUNSUPPORTED for batches whose plan does not fit a
+ * workgroup's LDS: total_tokens * q_heads / kv_heads / 256 + 2 * batch above 6000 may be. */
 uint64_t miikv_chunk_workspace_bytes(const miikv_view* view, uint32_t q_heads, uint32_t batch, uint32_t total_tokens,
                                      uint32_t max_tokens, uint32_t max_context, uint32_t window, uint32_t sinks);
 miikv_status miikv_chunk_attn(const miikv_view* view, const void* q, uint32_t q_dtype, uint32_t q_heads, float scale,

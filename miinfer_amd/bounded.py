@@ -170,7 +170,7 @@ def window_attention(cache: KvCache, q: torch.Tensor, scale: float | None = None
     _u32_arg("sinks", sinks)
     _u32_arg("max_context", max_context, 1)
     with _on_device(cache.k_codes.device):
-        if workspace is None or out is None:
+        if workspace is None or out is None or (gate is not None and gated_out is None):
             with _on_stream(stream):
                 if workspace is None:
                     workspace = _workspace(window_workspace_bytes(cache, q_heads, batch, tokens, max_context, window, sinks), q)
@@ -202,7 +202,7 @@ def scored_attention(cache: KvCache, q: torch.Tensor, key_weights: torch.Tensor,
     _u32_arg("max_context", max_context, 1)
     _check_weights("key_weights", key_weights, batch, cache.kv_heads, max_context)
     with _on_device(cache.k_codes.device):
-        if workspace is None or out is None:
+        if workspace is None or out is None or (gate is not None and gated_out is None):
             with _on_stream(stream):
                 if workspace is None:
                     workspace = _workspace(scored_workspace_bytes(cache, q_heads, batch, tokens, max_context), q)

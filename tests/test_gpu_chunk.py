@@ -290,6 +290,54 @@ def test_chunk_graphs_streams_and_equal_bits(gpu):
     assert torch.equal(got[:160], outs[0][:160])
 
 
+def test_chunk_many_rows_graph_and_two_streams(gpu):
+    """A captured call over expanded keys, replayed with other offsets and lengths, some of them few rows;
+    two calls at once on streams and workspaces of their own; out over q."""
+    import miinfer_amd as m
+    rng = np.random.default_rng(8)
+    hq, hk, d, cap, total = 32, 2, 128, 1024, 300
+    full = [1000, 300]
+    cache = paged(gpu, rng, hk, d, full, width=cap // 64)
+    q = _query(rng, gpu, (total, hq, d), torch.bfloat16)
+    off = _dev(np.array([0, 150, 300], np.int32), gpu)
+    lens = _dev(np.array(full, np.int32), gpu)
+
+    def room():
+        return torch.empty(m.chunk_workspace_bytes(cache, hq, 2, total, 200, cap, 300, 4), dtype=torch.uint8, device=gpu)
+
+    def step(out, ws, x=q, stream=None):
+        return m.chunk_attention(cache, x, off, lens, max_tokens=200, max_context=cap, window=300, sinks=4, out=out, workspace=ws,
+                                 stream=stream)
+
+    out, ws = torch.zeros_like(q), room()
+    step(out, ws)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step(out, ws)
+    for o, n in (([0, 150, 300], full), ([0, 1, 9], [700, 8]), ([0, 0, 200], [5, 290]), ([0, 150, 300], full)):
+        off.copy_(torch.tensor(o, dtype=torch.int32))
+        lens.copy_(torch.tensor(n, dtype=torch.int32))
+        out.fill_(3.0)
+        g.replay()
+        torch.cuda.synchronize()
+        want = step(torch.full_like(q, 3.0), room())
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        _check(cache, q[:o[2]], want[:o[2]], np.diff(o).tolist(), n, 300, 4)
+        assert bool((want[o[2]:] == 3).all())
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    spaces, outs = [room() for _ in streams], [torch.empty_like(q) for _ in streams]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for s, w, o in zip(streams, spaces, outs):
+            step(o, w, stream=s)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], out) and torch.equal(outs[1], out)
+    x = q.clone()
+    assert torch.equal(step(x, ws, x=x), out)
+
+
 def test_chunk_agrees_with_window_decode(gpu):
     """Chunks of one token are the decode form's rows."""
     import miinfer_amd as m

@@ -224,6 +224,23 @@ def test_part_graphs_share_a_workspace(gpu, scored):
             assert torch.equal(weights, want_w)
 
 
+def test_gated_output_is_made_when_all_else_is_given(gpu):
+    import miinfer_amd as m
+    rng = np.random.default_rng(21)
+    cache = paged(gpu, rng, 8, 128, [100])
+    q = _dev(_query(rng, (1, 32, 128), False), gpu)
+    gate = torch.randn(q.shape, device=gpu)
+    lens = _dev(np.array([100], np.int32), gpu)
+    w = torch.zeros((1, 8, 128), device=gpu)
+    out, both = m.window_attention(cache, q, window=0, lengths=lens, max_context=128, gate=gate)
+    assert out is None
+    ws = torch.empty(m.scored_workspace_bytes(cache, 32, 1, 1, 128), dtype=torch.uint8, device=gpu)
+    for call in (lambda **o: m.window_attention(cache, q, window=0, **o), lambda **o: m.scored_attention(cache, q, w, **o)):
+        out, gated = call(lengths=lens, max_context=128, gate=gate, out=torch.empty(q.shape, device=gpu), workspace=ws)
+        assert torch.equal(gated, both)
+        assert float((out * torch.sigmoid(gate) - gated).abs().max()) <= 1e-5
+
+
 def test_part_other_stream(gpu):
     import miinfer_amd as m
     rng = np.random.default_rng(10)
