@@ -79,17 +79,6 @@ __device__ __forceinline__ void load_weights(const float* w, uint32_t first, uin
     for (uint32_t j = 0; j < kPer; ++j) key[j] = first + j * 64 < hi ? ordered(x[j]) : 0u;
 }
 
-// Sum over the lanes up to this one.
-__device__ __forceinline__ uint32_t sum_to_lane(uint32_t x) {
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x111, 0xf, 0xf, true);  // row_shr:1, 2, 4, 8
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x112, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x114, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x118, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x142, 0xa, 0xf, true);  // row_bcast:15, to rows 1 and 3
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x143, 0xc, 0xf, true);  // row_bcast:31, to rows 2 and 3
-    return x;
-}
-
 __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictArgs a) {
     const uint32_t h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);

@@ -34,6 +34,17 @@ __host__ __device__ __forceinline__ Visible visible_steps(uint32_t L, uint32_t t
     return v;
 }
 
+// Sum over the lanes up to this one.
+__device__ __forceinline__ uint32_t sum_to_lane(uint32_t x) {
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x111, 0xf, 0xf, true);  // row_shr:1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x142, 0xa, 0xf, true);  // row_bcast:15, to rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x143, 0xc, 0xf, true);  // row_bcast:31, to rows 2 and 3
+    return x;
+}
+
 // The most steps that a context of at most max_context keys can have.
 inline uint32_t most_visible_steps(uint32_t max_context, uint32_t tokens, uint32_t window, uint32_t sinks) {
     const uint64_t all = (static_cast<uint64_t>(max_context) + kChunk - 1) / kChunk;

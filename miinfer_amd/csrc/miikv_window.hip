@@ -19,9 +19,9 @@
 // scale so far leaves below 2^15 (values of 0.02: outputs 4.5e-7 off; with a shift of 6 they
 // were 3.4e-6 to 4.9e-6 off).
 //
-// Work: the visible 32-key steps of all sequences are cut into runs of 4 * cpw steps, one
-// workgroup (of four waves) each.  cpw is chosen on the device from the lengths, so that
-// the runs of a ragged batch fill the chip whatever the lengths are.  A workgroup writes one record (o, m, l)
+// Work: the visible 32-key steps of all sequences are cut into runs, one workgroup (of four
+// waves) each, as many as the chip holds.  Their length is chosen on the device from the
+// lengths, so that the runs of a ragged batch fill the chip whatever the lengths are.  A workgroup writes one record (o, m, l)
 // per run; the second launch merges the records and, for weights, turns the kept scores
 // into probabilities with the merged m and l.
 #include "miikv_part.hpp"
@@ -53,7 +53,6 @@ struct PartArgs {
     uint32_t window;
     uint32_t sinks;
     uint32_t batch;
-    uint32_t target_wgs;
     uint32_t* runs;  // [batch][kv_heads][2]: first record and records of a pair that has any
     float* part;     // a record per run: o [cols][D], r [cols], l [cols], padded to 4, where
                      // o = sum of 2^(s - r) v and l = sum of 2^(s - r)
@@ -85,59 +84,71 @@ struct Run {
     bool live;
 };
 
-// Steps per wave: all sequences' steps over the target, by every wave for itself.
-__device__ __forceinline__ uint32_t steps_per_wave(const PartArgs& a) {
-    const uint32_t lane = threadIdx.x & 63;
-    unsigned long long sum = 0;
-    for (uint32_t b = lane; b < a.batch; b += 64) sum += part_steps(a, b);
-#pragma unroll
-    for (uint32_t off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off, 64);
-    const unsigned long long per = (sum * a.g.kv_heads + a.target_wgs * kWaves - 1) / (a.target_wgs * kWaves);
-    return per < 1 ? 1u : static_cast<uint32_t>(per);
+__device__ __forceinline__ uint32_t lane_of(uint32_t x, uint32_t lane) {
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), static_cast<int>(lane)));
 }
 
 // The run of workgroup w (all lanes take part, the result is wave-uniform).  In the order
-// (sequence, kv head, split), sequence b has kv_heads * ceil(steps / (kWaves * cpw)) runs.
+// (sequence, kv head, split), sequence b has kv_heads * runs_of(its steps) runs.
 __device__ __forceinline__ Run find_run(const PartArgs& a, uint32_t w) {
-    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t lane = threadIdx.x & 63, heads = a.g.kv_heads;
     Run r{};
-    if (a.batch == 1) {
-        const uint32_t n = part_steps(a, 0);
-        const uint32_t quota = kWaves * max(1u, (n * a.g.kv_heads + a.target_wgs * kWaves - 1) / (a.target_wgs * kWaves));
-        r.runs = __builtin_amdgcn_readfirstlane((n + quota - 1) / quota);
-        r.live = w < r.runs * a.g.kv_heads;
-        if (r.live) {
-            r.h = w / r.runs;
-            r.split = w - r.h * r.runs;
-        }
-        return r;
+    unsigned long long sum = 0;
+    uint32_t mine = 0;  // steps of sequence `lane`
+    if (a.batch <= 64) {
+        mine = lane < a.batch ? part_steps(a, lane) : 0u;
+        sum = lane_of(sum_to_lane(mine), 63);  // (64 contexts of at most 2^26 steps, not all of them that long)
+    } else {
+        for (uint32_t b = lane; b < a.batch; b += 64) sum += part_steps(a, b);
+#pragma unroll
+        for (uint32_t off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off, 64);
     }
-    const uint32_t quota = kWaves * steps_per_wave(a);
+    sum *= heads;
+    // The longest run, in sixteenths of a step: as short as leaves no more runs than slots, a step per wave at
+    // least.  (Multiples of four steps left a quarter of the slots empty or a few runs for a second round: 4
+    // sequences of 4 tokens 26.7 and 25.0 us.  Shorter runs for the workgroups that the CUs get second, which end
+    // later, were slower: 24.3 and 25.8 us for one sequence of 32768 keys.)
+    const unsigned long long share = (sum * 16 + kTargetWgs - 1) / kTargetWgs;
+    const uint32_t even = share < 0x3fffffffull ? static_cast<uint32_t>(share) : 0x3fffffffu;
+    uint32_t most = max(even, 16 * kWaves), n = 0, total = 0;
+    auto runs_of = [&](uint32_t steps) { return (16 * steps + most - 1) / most; };
+    if (a.batch <= 64) {
+        for (uint32_t x = 0;; ++x) {
+            n = runs_of(mine) * heads;
+            total = lane_of(sum_to_lane(n), 63);
+            if (total <= kTargetWgs || x == 16) break;
+            most = max(even + even / 16 * (x + 1) + 1, 16 * kWaves);
+        }
+    } else {
+        for (uint32_t b = lane; b < a.batch; b += 64) total += runs_of(part_steps(a, b)) * heads;
+        total = lane_of(sum_to_lane(total), 63);
+    }
+    if (w >= total) return r;
     uint32_t base = 0;
     for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
-        const uint32_t n = b0 + lane < a.batch ? (part_steps(a, b0 + lane) + quota - 1) / quota : 0u;
-        const uint32_t mine = n * a.g.kv_heads;
-        uint32_t incl = mine;
-#pragma unroll
-        for (uint32_t off = 1; off < 64; off <<= 1) {
-            const uint32_t up = __shfl_up(incl, off, 64);
-            if (lane >= off) incl += up;
-        }
-        const uint32_t before = base + incl - mine;
-        const unsigned long long at = __ballot(w >= before && w < before + mine);
-        if (at != 0) {
-            const int src = __builtin_ctzll(at);
-            const uint32_t x = w - __builtin_amdgcn_readfirstlane(__shfl(before, src, 64));
-            r.runs = __builtin_amdgcn_readfirstlane(__shfl(n, src, 64));
-            r.b = b0 + static_cast<uint32_t>(src);
-            r.h = x / r.runs;
+        if (a.batch > 64) n = b0 + lane < a.batch ? runs_of(part_steps(a, b0 + lane)) * heads : 0u;
+        const uint32_t upto = base + sum_to_lane(n);
+        const unsigned long long behind = __ballot(w < upto);
+        if (behind != 0) {
+            const uint32_t src = static_cast<uint32_t>(__builtin_ctzll(behind));
+            const uint32_t all = lane_of(n, src), x = w - (lane_of(upto, src) - all);
+            r.runs = __builtin_amdgcn_readfirstlane(all / heads);
+            r.b = b0 + src;
+            r.h = __builtin_amdgcn_readfirstlane(x / r.runs);
             r.split = x - r.h * r.runs;
             r.live = true;
             return r;
         }
-        base = __shfl(base + incl, 63, 64);
+        base = lane_of(upto, 63);
     }
     return r;
+}
+
+// The first step of a pair's k-th run: its steps are cut evenly into its runs.
+__device__ __forceinline__ uint32_t run_begin(uint32_t steps, uint32_t k, uint32_t runs) {
+    const uint64_t at = static_cast<uint64_t>(steps) * k;
+    if (at <= 0xffffffffu) return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at) / runs);
+    return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at / runs));
 }
 
 // Records of (b, h), which the first launch has noted for pairs that see any key.
@@ -183,10 +194,7 @@ part_kernel(PartArgs a) {
     const Geo& geo = a.g;
     const uint32_t L = part_length(a, b);
     const Visible vis = visible_steps(L, a.tokens, a.window, a.sinks);
-    // The pair's steps are cut evenly into its runs.
-    const uint32_t steps = vis.steps();
-    const uint32_t from = static_cast<uint32_t>(static_cast<uint64_t>(steps) * run.split / run.runs);
-    const uint32_t to = static_cast<uint32_t>(static_cast<uint64_t>(steps) * (run.split + 1) / run.runs);
+    const uint32_t from = run_begin(vis.steps(), run.split, run.runs), to = run_begin(vis.steps(), run.split + 1, run.runs);
     if (run.split == 0 && threadIdx.x == 0)
         *reinterpret_cast<uint2*>(a.runs + 2 * (static_cast<size_t>(b) * geo.kv_heads + h)) = make_uint2(blockIdx.x, run.runs);
 
@@ -657,7 +665,7 @@ PartPlan part_plan(const miikv_view* v, uint32_t q_heads, uint32_t batch, uint32
     PartPlan p{};
     const uint64_t pairs = static_cast<uint64_t>(batch) * v->kv_heads;
     const uint64_t most = most_visible_steps(max_context, tokens, window, sinks);
-    // the runs: at most the target and one partial run per pair, or one step per wave
+    // the runs: at most the slots and one partial run per pair, or one step per wave
     p.wgs = std::min<uint64_t>(kTargetWgs + pairs, pairs * ((most + kWaves - 1) / kWaves));
     const uint32_t cols = q_heads / v->kv_heads * tokens;
     p.run_bytes = up256(pairs * 2 * sizeof(uint32_t));
@@ -727,7 +735,6 @@ miikv_status part_impl(const miikv_view* view, const void* q, uint32_t q_dtype, 
     a.window = window;
     a.sinks = sinks;
     a.batch = batch;
-    a.target_wgs = kTargetWgs;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     a.runs = reinterpret_cast<uint32_t*>(ws);
     a.part = reinterpret_cast<float*>(ws + p.run_bytes);
