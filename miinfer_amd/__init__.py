@@ -1,6 +1,6 @@
 """miinfer_amd — MI355X-native quantized KV-cache path (q8_0 append, split-K GQA
-decode attention, suffix attention, prefix-state reuse) behind the C ABI in
-include/miikv.h.  This package is the host-side mirror of the reference's
+decode attention, suffix attention, attention over part of a cache and eviction,
+prefix-state reuse) behind the C ABI in include/miikv.h.  This package is the host-side mirror of the reference's
 KV-cache / attention call surface; all compute runs in libmiikv.so (HIP,
 gfx950) and fails loudly when that library is missing.
 """
