@@ -12,7 +12,7 @@
 //
 // In place, position i's source is at or behind i, so rows that go forward in order never
 // overwrite one that is still to move: a workgroup owns a slice of every row (some bytes of
-// each token, which no other workgroup touches), reads kMoveTokens tokens, waits until all of
+// each token, which no other workgroup touches), reads kMoveInPlace tokens, waits until all of
 // them have arrived, and writes them.  To other pages every tile is independent.
 //
 // Bound: the cache's lines that hold a kept row.  A K line of 128 bytes holds 8 tokens'
@@ -30,7 +30,10 @@ constexpr uint32_t kSelectThreads = 1024;
 constexpr uint32_t kSelectWaves = kSelectThreads / 64;
 constexpr uint32_t kCopies = 16;  // histograms, one per lane % 16: weights share their top digits
 constexpr uint32_t kCopyStride = kCopies + 1;  // words from a digit's counts to the next one's; odd, for the sums' reads
-constexpr uint32_t kMoveTokens = 256;     // destination tokens moved at a time
+constexpr uint32_t kMoveTokens = 256;    // destination tokens moved at a time, to other pages
+// In place, one turn after another.  (16384 keys of 8 heads to 4096, select and move: 256 at a time in slices of two
+// runs and 32 dims 54.5 us; 1024 at a time 36.7; and slices of one run and 8 dims 23.3.)
+constexpr uint32_t kMoveInPlace = 1024;
 
 struct EvictArgs {
     Geo g;
@@ -215,14 +218,21 @@ __device__ __forceinline__ uint32_t row_of(const Geo& g, const int32_t* table, u
     return (page * g.kv_heads + h) * g.page_tokens + tp;
 }
 
-// Roles of a (sequence, kv head)'s workgroups: D / 32 slices of K (4 runs of 8 + 8 dims),
-// D / 32 of V (32 dims), one of the scales.
+// Roles of a (sequence, kv head)'s workgroups: slices of K (one or two of a token's D / 16 runs of 8 + 8 dims), of
+// V (8 or 32 dims), one of the scales.  In place, where a workgroup moves all tokens of its slice, slices are
+// the smaller ones.
+template <uint32_t D, bool INPLACE>
+struct Roles {
+    static constexpr uint32_t k_runs = INPLACE ? 1 : 2, v_dims = INPLACE ? 8 : 32;
+    static constexpr uint32_t k = D / 16 / k_runs, v = D / v_dims, all = k + v + 1;
+};
 template <uint32_t D, bool KF16, bool VF16, bool INPLACE>
-__global__ void __launch_bounds__(kMoveTokens) move_kernel(EvictArgs a) {
+__global__ void __launch_bounds__(INPLACE ? kMoveInPlace : kMoveTokens) move_kernel(EvictArgs a) {
     constexpr uint32_t NB = D / 32;
-    constexpr uint32_t kRoles = 2 * (D / 64) + NB + 1;
+    using Role = Roles<D, INPLACE>;
     constexpr uint32_t KE = KF16 ? 2 : 1;
-    const uint32_t role = blockIdx.x % kRoles, tile = blockIdx.x / kRoles;
+    constexpr uint32_t kTok = INPLACE ? kMoveInPlace : kMoveTokens;
+    const uint32_t role = blockIdx.x % Role::all, tile = blockIdx.x / Role::all;
     const uint32_t h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
     const uint32_t left = min(evict_length(a, b), a.budget);
     if (!INPLACE && tile == 0 && role == 0 && h == 0 && tid == 0) a.new_lengths[b] = left;
@@ -230,9 +240,9 @@ __global__ void __launch_bounds__(kMoveTokens) move_kernel(EvictArgs a) {
     const int32_t* src_table = a.g.layout == MIIKV_LAYOUT_PAGED ? a.g.table + static_cast<size_t>(b) * a.g.table_stride : nullptr;
     const int32_t* dst_table = INPLACE ? src_table : a.dst_table + static_cast<size_t>(b) * a.dst_stride;
     // Two buffers: a wave may write the next tile's rows while another still stores this one's.
-    __shared__ uint32_t s_rows[2][2][kMoveTokens];
+    __shared__ uint32_t s_rows[2][2][kTok];
     uint32_t turn = 0;
-    for (uint32_t t0 = tile * kMoveTokens; t0 < left; t0 += kMoveTokens, turn ^= 1) {
+    for (uint32_t t0 = tile * kTok; t0 < left; t0 += kTok, turn ^= 1) {
         uint32_t *s_src = s_rows[turn][0], *s_dst = s_rows[turn][1];
         const uint32_t i = t0 + tid;
         bool moves = false;
@@ -243,16 +253,16 @@ __global__ void __launch_bounds__(kMoveTokens) move_kernel(EvictArgs a) {
             s_dst[tid] = row_of(a.g, dst_table, i, h);
         }
         if (!__syncthreads_or(moves) && INPLACE) continue;  // nothing of this tile moves
-        const uint32_t count = min(kMoveTokens, left - t0);
-        if (role < 2 * (D / 64)) {
-            // token tid's runs of 16 * KE bytes: chunk c = role / 2, g = 2 (role % 2) + 0, 1
-            u4v r[2][KE];
-            const size_t off = static_cast<size_t>(role / 2) * 1024 + (role % 2) * 512;
+        const uint32_t count = min(kTok, left - t0);
+        if (role < Role::k) {
+            // token tid's runs of 16 * KE bytes, k_runs from number role * k_runs on: of chunk c = number / 4, g = number % 4
+            u4v r[Role::k_runs][KE];
+            const size_t off = static_cast<size_t>(role) * Role::k_runs * 256;
             if (tid < count) {
                 const size_t row = s_src[tid];
                 const int8_t* p = a.g.k_codes + KE * ((row & ~size_t{15}) * D + off + (row & 15) * 16);
 #pragma unroll
-                for (uint32_t u = 0; u < 2; ++u)
+                for (uint32_t u = 0; u < Role::k_runs; ++u)
 #pragma unroll
                     for (uint32_t e = 0; e < KE; ++e) r[u][e] = *reinterpret_cast<const u4v*>(p + KE * u * 256 + 16 * e);
             }
@@ -264,21 +274,21 @@ __global__ void __launch_bounds__(kMoveTokens) move_kernel(EvictArgs a) {
                 const size_t row = s_dst[tid];
                 int8_t* p = a.g.k_codes + KE * ((row & ~size_t{15}) * D + off + (row & 15) * 16);
 #pragma unroll
-                for (uint32_t u = 0; u < 2; ++u)
+                for (uint32_t u = 0; u < Role::k_runs; ++u)
 #pragma unroll
                     for (uint32_t e = 0; e < KE; ++e) *reinterpret_cast<u4v*>(p + KE * u * 256 + 16 * e) = r[u][e];
             }
-        } else if (role < 2 * (D / 64) + NB) {
-            // 8 groups of 32 tokens x 32 dims x 4 units of 8 tokens (16 (x / 4) + 4 G + x % 4)
+        } else if (role < Role::k + Role::v) {
+            // groups of 32 tokens x v_dims dims x 4 units of 8 tokens (16 (x / 4) + 4 G + x % 4)
             using Elem = typename std::conditional<VF16, uint16_t, uint8_t>::type;
             constexpr uint32_t kPer = VF16 ? 2 : 4;  // elements of a 32-bit word
-            const uint32_t d0 = (role - 2 * (D / 64)) * 32;
+            const uint32_t d0 = (role - Role::k) * Role::v_dims;
             const Elem* v = reinterpret_cast<const Elem*>(a.g.v_codes);
-            constexpr uint32_t kUnits = 32 / 8;  // per thread
+            constexpr uint32_t kUnits = Role::v_dims / 8;  // per thread
             uint32_t r[kUnits][8 / kPer];
 #pragma unroll
             for (uint32_t j = 0; j < kUnits; ++j) {
-                const uint32_t x = j * kMoveTokens + tid, G = x & 3, d = d0 + ((x >> 2) & 31), H = x >> 7;
+                const uint32_t x = j * kTok + tid, G = x & 3, d = d0 + x / 4 % Role::v_dims, H = x / (4 * Role::v_dims);
 #pragma unroll
                 for (uint32_t k = 0; k < 8; ++k) {
                     const uint32_t t = min(32 * H + 16 * (k / 4) + 4 * G + k % 4, count - 1);
@@ -295,7 +305,7 @@ __global__ void __launch_bounds__(kMoveTokens) move_kernel(EvictArgs a) {
             }
 #pragma unroll
             for (uint32_t j = 0; j < kUnits; ++j) {
-                const uint32_t x = j * kMoveTokens + tid, G = x & 3, d = d0 + ((x >> 2) & 31), H = x >> 7;
+                const uint32_t x = j * kTok + tid, G = x & 3, d = d0 + x / 4 % Role::v_dims, H = x / (4 * Role::v_dims);
                 if (32 * H + 4 * G >= count) continue;
                 const size_t row = s_dst[32 * H];  // a group's rows are consecutive
                 Elem* to = reinterpret_cast<Elem*>(a.g.v_codes) + row * D + d * 32 + G * 8;
@@ -344,9 +354,9 @@ template <uint32_t D>
 void launch_move(const EvictArgs& a, bool kf, bool vf, hipStream_t s) {
     const uint32_t most = a.max_context < a.budget ? a.max_context : a.budget;
     const uint32_t tiles = a.dst_table != nullptr ? (most + kMoveTokens - 1) / kMoveTokens : 1u;
-    const dim3 grid((2 * (D / 64) + D / 32 + 1) * tiles, a.g.kv_heads, a.batch);
     const auto go = [&](auto k, auto v, auto in) {
-        hipLaunchKernelGGL((move_kernel<D, decltype(k)::value, decltype(v)::value, decltype(in)::value>), grid, dim3(kMoveTokens), 0, s, a);
+        const dim3 grid(Roles<D, decltype(in)::value>::all * tiles, a.g.kv_heads, a.batch);
+        hipLaunchKernelGGL((move_kernel<D, decltype(k)::value, decltype(v)::value, decltype(in)::value>), grid, dim3(decltype(in)::value ? kMoveInPlace : kMoveTokens), 0, s, a);
     };
     const auto with_in = [&](auto k, auto v) { a.dst_table == nullptr ? go(k, v, std::true_type{}) : go(k, v, std::false_type{}); };
     const auto with_v = [&](auto k) { vf ? with_in(k, std::true_type{}) : with_in(k, std::false_type{}); };
