@@ -461,6 +461,7 @@ miikv_status miikv_decode_attn_scored(const miikv_view* view, const void* q, uin
  *                 May be key_weights (with the same stride): what lay between the new
  *                 and the old length is zeroed then.  Otherwise entries past the new
  *                 length stay as they are.
+ *                 Memory that overlaps key_weights in another way is refused.
  * Rows of the cache past the new length stay as they were (in place: as the move left
  * them).  No counterpart in the reference. */
 miikv_status miikv_evict(const miikv_view* view, const float* key_weights, uint64_t weight_stride, uint32_t batch,

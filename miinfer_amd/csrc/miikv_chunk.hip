@@ -1082,7 +1082,7 @@ int chunk_plan(const miikv_view* v, uint32_t q_heads, uint32_t batch, uint32_t t
     if (max_tokens > total_tokens || max_tokens > max_context) return MIIKV_EINVAL;
     if (v->layout == MIIKV_LAYOUT_CONTIGUOUS && batch != 1) return MIIKV_EINVAL;
     const uint64_t rows = static_cast<uint64_t>(total_tokens) * (q_heads / v->kv_heads);
-    if (rows > 0x7fffffffu || batch > 65535u || v->kv_heads > 65535u) return MIIKV_EUNSUPPORTED;
+    if (rows > 0x7fffffffu || static_cast<uint64_t>(total_tokens) * q_heads > 0x7fffffffu || batch > 65535u || v->kv_heads > 65535u) return MIIKV_EUNSUPPORTED;
     // every sequence's last item may be a part of one
     p.items = std::min<uint64_t>(rows / kRows + batch, rows);
     p.steps = most_visible_steps(max_context, max_tokens, window, sinks);

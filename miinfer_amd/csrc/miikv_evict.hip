@@ -382,6 +382,11 @@ extern "C" miikv_status miikv_evict(const miikv_view* view, const float* key_wei
     const uint32_t most = max_context < budget ? max_context : budget;
     if (weights_out == key_weights ? weights_out_stride != weight_stride : weights_out != nullptr && weights_out_stride < most)
         return MIIKV_EINVAL;
+    if (weights_out != nullptr && weights_out != key_weights) {  // in place, or apart
+        const uint64_t rows = static_cast<uint64_t>(batch) * view->kv_heads - 1;
+        const uintptr_t in = reinterpret_cast<uintptr_t>(key_weights), to = reinterpret_cast<uintptr_t>(weights_out);
+        if (in < to + 4 * (rows * weights_out_stride + most) && to < in + 4 * (rows * weight_stride + max_context)) return MIIKV_EINVAL;
+    }
     if (dst_table != nullptr &&
         (view->layout != MIIKV_LAYOUT_PAGED || static_cast<uint64_t>(dst_stride) * view->page_tokens < most))
         return MIIKV_EINVAL;

@@ -103,6 +103,10 @@ def _evict(lib, v, **over):
     {"budget": 19}, {"sinks": 0xffffffff, "recent": 1}, {"kept": None}, {"new": None},
     {"dst": P, "dst_stride": 0}, {"dst": P, "dst_stride": 3, "budget": 769}, {"out": ctypes.c_void_p(0x20000), "out_stride": 255},
     {"out": P, "out_stride": 4000},
+    # weights over each other, not in place: behind the start, in the last row, in front and reaching in
+    {"out": ctypes.c_void_p(P.value + 4), "out_stride": 4096},
+    {"out": ctypes.c_void_p(P.value + 4 * (15 * 4096 + 4095)), "out_stride": 256},
+    {"out": ctypes.c_void_p(P.value - 4 * (15 * 256 + 255)), "out_stride": 256},
 ])
 def test_evict_refuses(over):
     L = _lib()
