@@ -414,7 +414,9 @@ miikv_status miikv_chunk_attn(const miikv_view* view, const void* q, uint32_t q_
  *   out / gated_out  device fp32, as q; gated_out = out * sigmoid(gate), gate and
  *        gated_out go together.  At least one output is required.
  * Outputs hold fp32's precision: key codes enter exactly, block scales are applied in
- * fp32, an fp32 query and the probabilities as two fp16 parts.  All pointers 16-byte
+ * fp32, an fp32 query and the probabilities as two fp16 parts.  What no token of the
+ * call sees may hold anything; a value that is not finite, in a key that only the later
+ * of several tokens see, may spread to the earlier ones.  All pointers 16-byte
  * aligned (else MIIKV_EINVAL).  The workspace needs no initialisation; calls that may
  * overlap need workspaces of their own.  miikv_window_workspace_bytes() is 0 for
  * arguments that the call refuses. */
