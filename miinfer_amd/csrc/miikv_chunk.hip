@@ -991,20 +991,22 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
 }
 
 // Merge of the items that were cut (9 to 12 us: two dependent reads, then up to 512 records of 64 or 128 KiB):
-// workgroup (item, kv head, 32 rows), 8 threads per row.
-constexpr uint32_t kMergeRows = 32;
+// workgroup (item, kv head, merge_rows<D> rows), D / 16 threads per row.
+template <uint32_t D>
+constexpr uint32_t merge_rows = 256 * 16 / D;
 template <uint32_t D>
 __global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs a) {
+    constexpr uint32_t kThreads = D / 16, kMergeRows = merge_rows<D>;
     const uint32_t i = blockIdx.x / (kRows / kMergeRows), h = blockIdx.y;
-    const uint32_t r = blockIdx.x % (kRows / kMergeRows) * kMergeRows + threadIdx.x / 8;
+    const uint32_t r = blockIdx.x % (kRows / kMergeRows) * kMergeRows + threadIdx.x / kThreads, part = threadIdx.x % kThreads;
     const ChunkItem it = a.items[i];  // (of nothing behind the last one: read with `head`, not after it)
     const uint32_t items = a.head[0], units = a.head[1], quota = a.head[2];
     if (i >= items || it.steps == 0 || r >= it.rows) return;
     const uint32_t first = h * units + it.start + kItemCost;
-    const uint32_t w0 = first / quota, w1 = (first + it.last) / quota;
+    const uint32_t w0 = uniform(first / quota), w1 = uniform((first + it.last) / quota);
     if (w0 == w1) return;  // written whole
     const uint32_t tok = it.tok0 + (it.head0 + r) / a.group, head = h * a.group + (it.head0 + r) % a.group;
-    constexpr uint32_t kPer = D / 64;  // groups of 8 values per thread
+    constexpr uint32_t kPer = 2;  // groups of 8 values per thread
     constexpr uint32_t kDepth = 4;     // records read at a time
     float acc[kPer][8] = {};
     float m = -INFINITY, sum = 0.0f;
@@ -1013,12 +1015,15 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs a) {
         half8 o[kDepth][kPer];
 #pragma unroll
         for (uint32_t j = 0; j < kDepth; ++j) {
-            const uint32_t x = min(w + j, w1);
-            const size_t rec = static_cast<size_t>(2 * x + (first < x * quota ? 0u : 1u)) * kRows + r;
-            ml[j] = a.rec_ml[rec];
-            if (w + j > w1) ml[j] = make_float2(-INFINITY, 0.0f);
+            ml[j] = make_float2(-INFINITY, 0.0f);
 #pragma unroll
-            for (uint32_t k = 0; k < kPer; ++k) o[j][k] = *reinterpret_cast<const half8*>(a.rec_o + rec * D + 64 * k + 8 * (threadIdx.x % 8));
+            for (uint32_t k = 0; k < kPer; ++k) o[j][k] = half8{};
+            if (w + j <= w1) {
+                const size_t rec = static_cast<size_t>(2 * (w + j) + (first < (w + j) * quota ? 0u : 1u)) * kRows + r;
+                ml[j] = a.rec_ml[rec];
+#pragma unroll
+                for (uint32_t k = 0; k < kPer; ++k) o[j][k] = *reinterpret_cast<const half8*>(a.rec_o + rec * D + D / 2 * k + 8 * part);
+            }
         }
         float to = m;
 #pragma unroll
@@ -1042,13 +1047,13 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs a) {
             }
     }
     const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-    const size_t at = (static_cast<size_t>(tok) * a.q_heads + head) * D + 8 * (threadIdx.x % 8);
+    const size_t at = (static_cast<size_t>(tok) * a.q_heads + head) * D + 8 * part;
     with_type(a.out_dtype, [&](auto t) __attribute__((always_inline)) {
 #pragma unroll
         for (uint32_t k = 0; k < kPer; ++k)
 #pragma unroll
             for (uint32_t x = 0; x < 8; x += 4)
-                store4<decltype(t)>(a.out, at + 64 * k + x, make_float4(acc[k][x] * inv, acc[k][x + 1] * inv, acc[k][x + 2] * inv, acc[k][x + 3] * inv));
+                store4<decltype(t)>(a.out, at + D / 2 * k + x, make_float4(acc[k][x] * inv, acc[k][x + 1] * inv, acc[k][x + 2] * inv, acc[k][x + 3] * inv));
     });
 }
 
@@ -1117,7 +1122,7 @@ int launch_chunk(const ChunkArgs& a, const ChunkPlan& p, bool kf, bool vf, hipSt
     };
     const auto with_v = [&](auto k) { vf ? go(k, std::true_type{}) : go(k, std::false_type{}); };
     kf ? with_v(std::true_type{}) : with_v(std::false_type{});
-    hipLaunchKernelGGL((chunk_merge_kernel<D>), dim3(static_cast<uint32_t>(p.items) * (kRows / kMergeRows), a.g.kv_heads), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((chunk_merge_kernel<D>), dim3(static_cast<uint32_t>(p.items) * (kRows / merge_rows<D>), a.g.kv_heads), dim3(256), 0, s, a);
     return hip_status(hipGetLastError());
 }
 
