@@ -156,12 +156,7 @@ __device__ __forceinline__ Span span_of(const ChunkArgs& a, const Chunk& c, uint
 // Inclusive sums over the workgroup's threads; `total` is the last one's.
 __device__ __forceinline__ uint32_t scan_threads(uint32_t x, uint32_t* s_wave, uint32_t& total) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint32_t incl = x;
-#pragma unroll
-    for (uint32_t off = 1; off < 64; off <<= 1) {
-        const uint32_t up = __shfl_up(incl, off, 64);
-        if (lane >= off) incl += up;
-    }
+    const uint32_t incl = sum_to_lane(x);
     __syncthreads();
     if (lane == 63) s_wave[wave] = incl;
     __syncthreads();
