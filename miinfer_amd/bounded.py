@@ -17,7 +17,7 @@ import torch
 
 from . import _lib
 from ._lib import call, lib
-from .kv import KvCache, _on_stream, _ptr, _stream
+from .kv import KvCache, _on_stream, _ptr
 
 _INDEX = (torch.int32, torch.uint32)
 
@@ -29,6 +29,11 @@ def _on_device(dev: torch.device):
     if dev.index is None or dev.index == torch.cuda.current_device():
         return contextlib.nullcontext()
     return torch.cuda.device(dev)
+
+
+def _queue(dev: torch.device, stream) -> ctypes.c_void_p:
+    # (the device is named: current_stream() would look for it first, about 0.5 us of a call)
+    return ctypes.c_void_p((torch.cuda.current_stream(dev) if stream is None else stream).cuda_stream)
 
 
 def _check(cache: KvCache, stream, **tensors) -> None:
@@ -130,7 +135,8 @@ def chunk_attention(cache: KvCache, q: torch.Tensor, offsets: torch.Tensor, leng
     _u32_arg("max_context", max_context, 1)
     _u32_arg("window", window)
     _u32_arg("sinks", sinks)
-    with _on_device(cache.k_codes.device):
+    dev = cache.k_codes.device
+    with _on_device(dev):
         if workspace is None or out is None:
             with _on_stream(stream):
                 if workspace is None:
@@ -141,7 +147,7 @@ def chunk_attention(cache: KvCache, q: torch.Tensor, offsets: torch.Tensor, leng
         call("miikv_chunk_attn", cache.view, q.data_ptr(), _DTYPES[q.dtype], q_heads,
              1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale), batch, total, offsets.data_ptr(),
              lengths.data_ptr(), max_tokens, max_context, window, sinks, out.data_ptr(), _DTYPES[out.dtype],
-             workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(stream))
+             workspace.data_ptr(), workspace.numel() * workspace.element_size(), _queue(dev, stream))
     return out
 
 
@@ -169,7 +175,8 @@ def window_attention(cache: KvCache, q: torch.Tensor, scale: float | None = None
     _u32_arg("window", window)
     _u32_arg("sinks", sinks)
     _u32_arg("max_context", max_context, 1)
-    with _on_device(cache.k_codes.device):
+    dev = cache.k_codes.device
+    with _on_device(dev):
         if workspace is None or out is None or (gate is not None and gated_out is None):
             with _on_stream(stream):
                 if workspace is None:
@@ -178,7 +185,7 @@ def window_attention(cache: KvCache, q: torch.Tensor, scale: float | None = None
         call("miikv_decode_attn_window", cache.view, q.data_ptr(), 0 if q.dtype == torch.float16 else 1, q_heads,
              1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale), batch, tokens, _ptr(lengths),
              _ptr(decode_state), max_context, window, sinks, _ptr(out), _ptr(gate), _ptr(gated_out),
-             workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(stream))
+             workspace.data_ptr(), workspace.numel() * workspace.element_size(), _queue(dev, stream))
     return out, gated_out
 
 
@@ -201,7 +208,8 @@ def scored_attention(cache: KvCache, q: torch.Tensor, key_weights: torch.Tensor,
         max_context = cache.capacity
     _u32_arg("max_context", max_context, 1)
     _check_weights("key_weights", key_weights, batch, cache.kv_heads, max_context)
-    with _on_device(cache.k_codes.device):
+    dev = cache.k_codes.device
+    with _on_device(dev):
         if workspace is None or out is None or (gate is not None and gated_out is None):
             with _on_stream(stream):
                 if workspace is None:
@@ -210,7 +218,7 @@ def scored_attention(cache: KvCache, q: torch.Tensor, key_weights: torch.Tensor,
         call("miikv_decode_attn_scored", cache.view, q.data_ptr(), 0 if q.dtype == torch.float16 else 1, q_heads,
              1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale), batch, tokens, _ptr(lengths),
              _ptr(decode_state), max_context, key_weights.data_ptr(), key_weights.shape[2], _ptr(out), _ptr(gate),
-             _ptr(gated_out), workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(stream))
+             _ptr(gated_out), workspace.data_ptr(), workspace.numel() * workspace.element_size(), _queue(dev, stream))
     return out, gated_out
 
 
@@ -271,5 +279,5 @@ def evict(cache: KvCache, key_weights: torch.Tensor, lengths: torch.Tensor, *, b
                     new_lengths = torch.empty((batch,), dtype=torch.int32, device=dev)
         call("miikv_evict", cache.view, key_weights.data_ptr(), key_weights.shape[2], batch, lengths.data_ptr(), max_context,
              sinks, recent, budget, _ptr(dst_table), 0 if dst_table is None else dst_table.shape[1], kept.data_ptr(),
-             new_lengths.data_ptr(), _ptr(weights_out), 0 if weights_out is None else weights_out.shape[2], _stream(stream))
+             new_lengths.data_ptr(), _ptr(weights_out), 0 if weights_out is None else weights_out.shape[2], _queue(dev, stream))
     return kept, new_lengths
