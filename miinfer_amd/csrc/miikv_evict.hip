@@ -72,7 +72,8 @@ __device__ __forceinline__ uint32_t ordered(float w) {
 //
 // Bound: instructions of one compute unit, 256 cycles for each one that every key of 16384 needs,
 // and the latency of the two reads and the barriers.  (For 16384 keys of 8 heads: the weights read anew
-// in every pass, one at a time, 31.4 us; held in registers 19; so 12.8.)
+// in every pass, one at a time, 31.4 us; held in registers 19; a wave's keys one
+// behind another, weights moved from registers 12.8; passes left out where all that share the digits stay 12.0.)
 constexpr uint32_t kPer = 16;
 constexpr uint32_t kSegment = kPer * kSelectThreads;
 
@@ -115,7 +116,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictArgs a) {
         for (uint32_t i = tid; i < 4 * 256 * kCopyStride; i += kSelectThreads) (&s_hist[0][0])[i] = 0;
         load_weights(w, first, hi, x, key);
         __syncthreads();
-        uint32_t prefix = 0, k = need;
+        uint32_t prefix = 0, k = need, low = 0;  // the limit's digits so far; keys of them that stay; bits not looked at
 #pragma unroll
         for (uint32_t pass = 0; pass < 4; ++pass) {
             const uint32_t shift = 24 - 8 * pass;
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictArgs a) {
             }
             __syncthreads();
             // Every wave finds the digit.  Lane l: digits 255 - 4l down to 252 - 4l.
-            uint32_t c[4], sum = 0, digit = 0, before = 0;
+            uint32_t c[4], sum = 0, digit = 0, before = 0, here = 0;
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j) sum += c[j] = s_count[pass][255 - 4 * lane - j];
             uint32_t above = sum_to_lane(sum) - sum;
@@ -146,12 +147,18 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictArgs a) {
                 if (above < k) {
                     digit = 255 - 4 * lane - j;
                     before = above;
+                    here = c[j];
                 }
                 above += c[j];
             }
             const uint32_t from_lane = static_cast<uint32_t>(__builtin_ctzll(__ballot(mine)));
             prefix = prefix << 8 | static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(digit), from_lane));
             k -= static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(before), from_lane));
+            // All keys that share these digits stay: the others need not be told apart.
+            if (k == static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(here), from_lane))) {
+                low = shift;
+                break;
+            }
         }
         // Keys above `prefix` stay, and the first k of those equal to it.  In place, a weight's new
         // position is at or before its old one, and its segment has been read whole by then.
@@ -161,8 +168,8 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictArgs a) {
             uint32_t gt = 0, eq = 0;
 #pragma unroll
             for (uint32_t j = 0; j < kPer; ++j) {
-                gt += static_cast<uint32_t>(__popcll(__ballot(key[j] > prefix)));
-                eq += static_cast<uint32_t>(__popcll(__ballot(key[j] == prefix)));
+                gt += static_cast<uint32_t>(__popcll(__ballot((key[j] >> low) > prefix)));
+                eq += static_cast<uint32_t>(__popcll(__ballot((key[j] >> low) == prefix)));
             }
             if (lane == 0) s_total[turn][wave] = make_uint2(gt, eq);
             __syncthreads();
@@ -174,11 +181,11 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictArgs a) {
             eq0 += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(ei), 63));
 #pragma unroll
             for (uint32_t j = 0; j < kPer; ++j) {
-                const unsigned long long gts = __ballot(key[j] > prefix), eqs = __ballot(key[j] == prefix);
+                const unsigned long long gts = __ballot((key[j] >> low) > prefix), eqs = __ballot((key[j] >> low) == prefix);
                 if ((gts | eqs) != 0) {
                     const uint32_t eq_mine = eq_at + lanes_before(eqs);
                     const uint32_t to = a.sinks + gt_at + lanes_before(gts) + min(eq_mine, k);
-                    if (key[j] > prefix || (key[j] == prefix && eq_mine < k)) {
+                    if ((key[j] >> low) > prefix || ((key[j] >> low) == prefix && eq_mine < k)) {
                         kept[to] = static_cast<int32_t>(first + from + j * 64);
                         if (moves) out[to] = x[j];
                     }
