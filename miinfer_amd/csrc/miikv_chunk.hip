@@ -24,9 +24,9 @@
 // With many rows per sequence expand_kernel makes the fp16 tiles first, and the ring holds those.
 //
 // Bound: the matrix unit where rows are many (two 512-token chunks over 8704 keys, head_dim 256: this kernel
-// 190 us, 1.12 PFLOP/s, 61% of its cycles in MFMAs; prompts at head_dim 128: 142 us, 0.91 PFLOP/s, with half the
+// 196 us, 1.08 PFLOP/s, 61% of its cycles in MFMAs; prompts at head_dim 128: 152 us, 0.85 PFLOP/s, with half the
 // MFMAs for the same exponentials); where they are few, the conversions and what an item costs before its
-// first step and after its last (12 sequences of 3 to 39 tokens: 40 us).
+// first step and after its last (12 sequences of 3 to 39 tokens: 41 us).
 //
 // Precision: query, code * scale and probabilities are fp16, the matrix unit's operands, sums and
 // statistics fp32; the records' normalised outputs are fp16, half the bytes that the merge reads. Outputs are
@@ -271,7 +271,7 @@ __device__ __forceinline__ const half8* tile_at(const ChunkArgs& a, uint32_t b, 
 
 // One step of (sequence z, kv head y) as an fp16 tile: code * scale, rounded once.  Keys that no
 // token of the chunk sees may hold anything: their values become 0.
-// Bound: HBM (the codes once, the tiles once).
+// Bound: HBM (the codes once, the tiles once: two sequences of 8704 keys, head_dim 256, 105 MB in 23 us).
 template <uint32_t D, bool KF16, bool VF16>
 __global__ void __launch_bounds__(256) expand_kernel(ChunkArgs a) {
     constexpr uint32_t NB = D / 32, KE = KF16 ? 2 : 1, VE = VF16 ? 2 : 1, kRuns = 2 * D;  // 16 codes each, of K and of V
@@ -985,7 +985,7 @@ __global__ void __launch_bounds__(kChunkThreads) __attribute__((amdgpu_waves_per
     }
 }
 
-// Merge of the items that were cut (9 to 12 us: two dependent reads, then up to 512 records of 64 or 128 KiB):
+// Merge of the items that were cut (8 to 11 us: two dependent reads, then up to 512 records of 64 or 128 KiB):
 // workgroup (item, kv head, merge_rows<D> rows), D / 16 threads per row.
 template <uint32_t D>
 constexpr uint32_t merge_rows = 256 * 16 / D;

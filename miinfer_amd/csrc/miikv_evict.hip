@@ -73,7 +73,7 @@ __device__ __forceinline__ uint32_t ordered(float w) {
 // Bound: instructions of one compute unit, 256 cycles for each one that every key of 16384 needs,
 // and the latency of the two reads and the barriers.  (For 16384 keys of 8 heads: the weights read anew
 // in every pass, one at a time, 31.4 us; held in registers 19; a wave's keys one
-// behind another, weights moved from registers 12.8; passes left out where all that share the digits stay 12.0.)
+// behind another, weights moved from registers 12.8; passes left out where all that share the digits stay 12.1.)
 constexpr uint32_t kPer = 16;
 constexpr uint32_t kSegment = kPer * kSelectThreads;
 
