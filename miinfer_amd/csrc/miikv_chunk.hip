@@ -271,7 +271,7 @@ __device__ __forceinline__ const half8* tile_at(const ChunkArgs& a, uint32_t b, 
 
 // One step of (sequence z, kv head y) as an fp16 tile: code * scale, rounded once.  Keys that no
 // token of the chunk sees may hold anything: their values become 0.
-// Bound: HBM (the codes once, the tiles once: two sequences of 8704 keys, head_dim 256, 105 MB in 23 us).
+// Bound: HBM (the codes once, the tiles once: two sequences of 8704 keys, head_dim 256, 109 MB in 23 us).
 template <uint32_t D, bool KF16, bool VF16>
 __global__ void __launch_bounds__(256) expand_kernel(ChunkArgs a) {
     constexpr uint32_t NB = D / 32, KE = KF16 ? 2 : 1, VE = VF16 ? 2 : 1, kRuns = 2 * D;  // 16 codes each, of K and of V
