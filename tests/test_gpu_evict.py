@@ -165,6 +165,25 @@ def test_evict_long(gpu):
     _check(cache, before, w, kept, [n], new, 30000, 4, 1000)
 
 
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("mode", [0, 1, 2, 3])
+@pytest.mark.parametrize("budget", [1024, 1025, 3070])
+def test_evict_in_place_over_several_turns(gpu, d, mode, budget):
+    """More rows than move at a time, in place, where kept keys stand close and far apart: every plane, sequences of
+    which one stays as it is."""
+    import miinfer_amd as m
+    rng = np.random.default_rng(d + mode + budget)
+    lengths = [5001, 900, budget + 1]
+    cache = paged(gpu, rng, 2, d, lengths, mode=mode, page=128)
+    w = rng.random((3, 2, 5100)).astype(np.float32)
+    w[0, 0, :2500] += 1.0  # the front stays whole, then the rest moves far
+    w[0, 1, 2500:] += 1.0
+    before = [_rows(cache, b, n) for b, n in enumerate(lengths)]
+    kept, new = m.evict(cache, _dev(w, gpu), _dev(np.array(lengths, np.int32), gpu), budget=budget, sinks=3, recent=20,
+                        max_context=5100)
+    _check(cache, before, w, kept, lengths, new, budget, 3, 20)
+
+
 @pytest.mark.parametrize("n,budget,sinks,recent", [(16390, 9000, 4, 2), (16391, 9000, 4, 2), (40001, 21000, 0, 5000),
                                                    (40001, 39990, 7, 30000), (50000, 50, 25, 25), (33000, 32999, 0, 0)])
 @pytest.mark.parametrize("own_rows", [True, False])
